@@ -39,7 +39,8 @@ enum { TREAD_F32 = 0, TREAD_F16 = 1, TREAD_BF16 = 2 };
 const char* tread_last_error(void);
 
 /* ABI revision of this library; bumped on any signature change, new entry point or newly accepted flag
- * (4: tread_attn_rows accepts TREAD_ATTN_FORCE_TAIL_SPLIT; 5: tread_rows_gemm). */
+ * (4: tread_attn_rows accepts TREAD_ATTN_FORCE_TAIL_SPLIT; 5: tread_rows_gemm; 6: tread_paged_append,
+ * tread_paged_attn, tread_adjust_logits). */
 int tread_abi_version(void);
 
 /*
@@ -251,6 +252,81 @@ size_t tread_rows_gemm_workspace_bytes(void);
 int tread_rows_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, void* out,
                     int64_t ld_out, int M, int N, int K, int accumulate, int dtype, void* err_flag,
                     void* workspace, size_t workspace_bytes, tread_stream_t stream);
+
+/*
+ * Paged key-value cache: pools k_pages, v_pages of num_pages pages, each [Hkv, page_size, D] at
+ * head stride head_stride, pages page_stride apart (elements), so that one layer of a pool
+ * [num_pages, L, Hkv, page_size, D] is a pool too. Token t of sequence s lies in slot t % page_size
+ * of page table[s * table_ld + t / page_size]. Any page_size of at least 1. The reference has no
+ * counterpart: its decode loop concatenates every new token to the cache (tread/server.py:200-211).
+ *
+ * tread_paged_append writes the keys and values of R new tokens into their pages, rotating keys (and
+ * the rows' query heads) on the way:
+ *   k, v    : row r, head g at r * k_ld + g * k_sh (v_ld, v_sh), D consecutive elements: columns of a
+ *             fused projection, or a dense cache [Hkv, R, D]; q likewise (q_ld, q_sh), Hq = 0 without
+ *   q_out   : [R, Hq, D] contiguous; may be q itself
+ *   pos     : device int64 [R], the row's token position in its sequence; negative: a padding row,
+ *             which appends nothing and whose q_out row is zero
+ *   seq     : device int32 [R], the row's sequence (a row of table), or NULL: row r is sequence r
+ *   rope_pos: device int64 [R], |rope_pos| < 2^31, the position that the rotation uses, or NULL: pos.
+ *             A cached block that moves by some offset is re-rotated by that offset.
+ *   inv_freq: DEVICE fp32 [D/2], or NULL: keys are copied (then Hq = 0). The angle is
+ *             rope_pos * inv_freq in 64 bits; cos and sin times attn_scaling in fp32; rounded once.
+ * A row whose sequence, position or page id is out of range appends nothing, gets a q_out row of zeros
+ * and sets bit 0 of *err_flag (may be NULL). No two rows may name the same token; D even, at most 256.
+ */
+int tread_paged_append(const void* k, int64_t k_ld, int64_t k_sh, const void* v, int64_t v_ld, int64_t v_sh,
+                       const void* q, int64_t q_ld, int64_t q_sh, void* q_out, void* k_pages, void* v_pages,
+                       int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
+                       const int32_t* table, int64_t table_ld, int num_seqs, int max_pages,
+                       const int32_t* seq, const int64_t* pos, const int64_t* rope_pos, int R, int Hq,
+                       int Hkv, int D, const float* inv_freq, float attn_scaling, int dtype,
+                       void* err_flag, tread_stream_t stream);
+
+/*
+ * Attention of one new token per sequence over its pages (the attention of tread/server.py:207-209's
+ * decode forward): out[b, h] = softmax(sm_scale * q[b, h] . K[0..lens[b]-1, g]) V, g = h / (Hq / Hkv).
+ *   q     : [B, Hq, D], rows q_ld apart; out: [B, Hq, D] contiguous
+ *   table : device int32 [B, max_pages] at row stride table_ld; entries behind a sequence's last page
+ *           are not read
+ *   lens  : device int64 [B], keys of each sequence, the new token's own among them. Where no key has
+ *           a score above -inf, or there is none, the output is zero
+ * A length below 0 or above max_pages * page_size gives a row of zeros; keys in a page whose id is
+ * outside the pool count as masked. Both set bit 1 of *err_flag (may be NULL). What slots behind a
+ * sequence's length hold does not matter. D in {64, 128, 256}, Hq / Hkv at most 16.
+ * workspace: tread_paged_attn_workspace_bytes() of device memory, 256-byte aligned, contents
+ * irrelevant; calls that share one must be stream-ordered.
+ */
+size_t tread_paged_attn_workspace_bytes(int Hq, int Hkv, int D);
+int tread_paged_attn(const void* q, int64_t q_ld, const void* k_pages, const void* v_pages,
+                     int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
+                     const int32_t* table, int64_t table_ld, int max_pages, const int64_t* lens, int B,
+                     int Hq, int Hkv, int D, float sm_scale, void* out, int dtype, void* err_flag,
+                     void* workspace, size_t workspace_bytes, tread_stream_t stream);
+
+/*
+ * The next token's logits, adjusted (no counterpart in the reference, which is greedy on raw logits,
+ * tread/server.py:203,210). Per row b, with n the count of token v in tokens[b, prompt_lens[b] : lens[b]]:
+ *   x = logits[b, v];  if v is in tokens[b, 0 : lens[b]]: x = x > 0 ? x / repetition : x * repetition
+ *   x -= frequency * n + presence * (n > 0);  x += the biases of v;  v not allowed: x = -inf
+ * in fp32, rounded once to out_dtype.
+ *   logits, out : [B, V] at row strides ld, ld_out; out may be logits itself (same type and stride)
+ *   tokens      : device int64 [B, max_tokens] at row stride tokens_ld, or NULL; ids outside [0, V) count
+ *                 for nothing. lens: device int64 [B] or NULL (max_tokens); prompt_lens: NULL is 0
+ *   repetition, presence, frequency: device fp32 [B], or NULL: the value beside it for every row
+ *                 (repetition above 0)
+ *   bias_ids, bias: device int64 / fp32 [B, num_bias] at their row strides (0: one list for all rows);
+ *                 ids outside [0, V) count for nothing, several biases of one token add up in order
+ *   allowed     : device int32 [B, ceil(V / 32)] at row stride allowed_ld (0: one mask for all rows),
+ *                 bit v % 32 of word v / 32 set: v is allowed; NULL: every token is
+ */
+int tread_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, int B, int V,
+                        const int64_t* tokens, int64_t tokens_ld, int max_tokens, const int64_t* lens,
+                        const int64_t* prompt_lens, const float* repetition, float repetition_all,
+                        const float* presence, float presence_all, const float* frequency,
+                        float frequency_all, const int64_t* bias_ids, int64_t bias_ids_ld,
+                        const float* bias, int64_t bias_ld, int num_bias, const int32_t* allowed,
+                        int64_t allowed_ld, int dtype, int out_dtype, tread_stream_t stream);
 
 /*
  * Block-store tier transfers (pinned host <-> HBM), stream-ordered DMA copies.

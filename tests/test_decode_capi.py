@@ -1,0 +1,77 @@
+"""Host-side argument checks of the decode-step entry points (no GPU: nothing is launched)."""
+import pytest
+
+from tread_b200 import _capi as C
+
+
+def _append_call(**over):
+    a = dict(k=256, k_ld=1024, k_sh=128, v=256, v_ld=1024, v_sh=128, q=256, q_ld=1024, q_sh=128, q_out=256, kp=256,
+             vp=256, ps=2 * 16 * 128, hs=16 * 128, N=8, page=16, table=256, t_ld=4, S=4, P=4, seq=None, pos=256,
+             rpos=None, R=3, Hq=4, Hkv=2, D=128, inv=256, scale=1.0, dtype=C.TREAD_BF16)
+    a.update(over)
+    return C.lib().tread_paged_append(
+        a["k"], a["k_ld"], a["k_sh"], a["v"], a["v_ld"], a["v_sh"], a["q"], a["q_ld"], a["q_sh"], a["q_out"], a["kp"],
+        a["vp"], a["ps"], a["hs"], a["N"], a["page"], a["table"], a["t_ld"], a["S"], a["P"], a["seq"], a["pos"],
+        a["rpos"], a["R"], a["Hq"], a["Hkv"], a["D"], a["inv"], a["scale"], a["dtype"], None, None)
+
+
+@pytest.mark.parametrize("over,needle", [
+    (dict(R=-1), "R < 0"), (dict(k=None), "null"), (dict(pos=None), "null"), (dict(Hkv=0), "heads"),
+    (dict(Hq=-1), "heads"), (dict(D=127), "head_dim"), (dict(D=258), "head_dim"), (dict(q=None), "query heads"),
+    (dict(inv=None), "query heads"), (dict(q_out=None), "query heads"), (dict(dtype=7), "dtype"),
+    (dict(page=0), "page geometry"), (dict(N=-1), "page geometry"), (dict(ps=100), "page geometry"),
+    (dict(hs=100), "page geometry"), (dict(table=None), "page table"), (dict(t_ld=3), "page table"),
+    (dict(R=5), "without seq"),
+])
+def test_paged_append_rejects_bad_arguments(over, needle):
+    assert _append_call(**over) == 1
+    assert needle in C.lib().tread_last_error().decode()
+
+
+def _attn_call(**over):
+    a = dict(q=256, q_ld=512, kp=256, vp=256, ps=2 * 16 * 128, hs=16 * 128, N=8, page=16, table=256, t_ld=4, P=4,
+             lens=256, B=3, Hq=4, Hkv=2, D=128, scale=0.1, out=256, dtype=C.TREAD_BF16, ws=256, ws_bytes=None)
+    a.update(over)
+    n = C.lib().tread_paged_attn_workspace_bytes(4, 2, 128) if a["ws_bytes"] is None else a["ws_bytes"]
+    return C.lib().tread_paged_attn(
+        a["q"], a["q_ld"], a["kp"], a["vp"], a["ps"], a["hs"], a["N"], a["page"], a["table"], a["t_ld"], a["P"],
+        a["lens"], a["B"], a["Hq"], a["Hkv"], a["D"], a["scale"], a["out"], a["dtype"], None, a["ws"], n, None)
+
+
+@pytest.mark.parametrize("over,needle", [
+    (dict(B=-1), "B < 0"), (dict(q=None), "null"), (dict(lens=None), "null"), (dict(Hq=3), "heads"),
+    (dict(Hq=34), "heads"), (dict(Hkv=0), "heads"), (dict(D=96), "head_dim"), (dict(dtype=9), "dtype"),
+    (dict(page=0), "page geometry"), (dict(hs=16), "page geometry"), (dict(table=None), "page table"),
+    (dict(t_ld=2), "page table"),
+])
+def test_paged_attn_rejects_bad_arguments(over, needle):
+    assert _attn_call(**over) == 1
+    assert needle in C.lib().tread_last_error().decode()
+
+
+def _logits_call(**over):
+    a = dict(x=256, ld=100, out=256, ld_out=100, B=2, V=100, tok=256, tok_ld=8, H=8, lens=256, plens=256, rep=None,
+             rep_all=1.2, pres=None, pres_all=0.0, freq=None, freq_all=0.0, ids=256, ids_ld=2, bias=256, bias_ld=2,
+             nb=2, allowed=256, al_ld=4, dtype=C.TREAD_BF16, odt=C.TREAD_F32)
+    a.update(over)
+    return C.lib().tread_adjust_logits(
+        a["x"], a["ld"], a["out"], a["ld_out"], a["B"], a["V"], a["tok"], a["tok_ld"], a["H"], a["lens"], a["plens"],
+        a["rep"], a["rep_all"], a["pres"], a["pres_all"], a["freq"], a["freq_all"], a["ids"], a["ids_ld"], a["bias"],
+        a["bias_ld"], a["nb"], a["allowed"], a["al_ld"], a["dtype"], a["odt"], None)
+
+
+@pytest.mark.parametrize("over,needle", [
+    (dict(B=-1), "B < 0"), (dict(x=None), "null"), (dict(out=None), "null"), (dict(dtype=5), "dtype"),
+    (dict(odt=5), "dtype"), (dict(ld=99), "row stride"), (dict(ld_out=99), "row stride"), (dict(H=-1), "history"),
+    (dict(tok_ld=7), "history"), (dict(bias=None), "biases"), (dict(nb=-1), "biases"), (dict(rep_all=0.0), "repetition"),
+    (dict(rep_all=float("nan")), "repetition"),
+])
+def test_adjust_logits_rejects_bad_arguments(over, needle):
+    assert _logits_call(**over) == 1
+    assert needle in C.lib().tread_last_error().decode()
+
+
+def test_empty_calls_are_noops():
+    assert _append_call(R=0) == 0
+    assert _attn_call(B=0) == 0
+    assert _logits_call(B=0) == 0 and _logits_call(V=0) == 0

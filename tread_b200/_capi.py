@@ -68,6 +68,22 @@ SIGNATURES = {
     ),
     "tread_rmsnorm": (ctypes.c_int, [P, I64, P, P, I64, I64, ctypes.c_int, F32, ctypes.c_int, P]),
     "tread_silu_mul": (ctypes.c_int, [P, I64, P, I64, I64, ctypes.c_int, ctypes.c_int, P]),
+    "tread_paged_append": (
+        ctypes.c_int,
+        [P, I64, I64, P, I64, I64, P, I64, I64, P, P, P, I64, I64, I64, ctypes.c_int, P, I64, ctypes.c_int,
+         ctypes.c_int, P, P, P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, P, F32, ctypes.c_int, P, P],
+    ),
+    "tread_paged_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "tread_paged_attn": (
+        ctypes.c_int,
+        [P, I64, P, P, I64, I64, I64, ctypes.c_int, P, I64, ctypes.c_int, P, ctypes.c_int, ctypes.c_int,
+         ctypes.c_int, ctypes.c_int, F32, P, ctypes.c_int, P, P, ctypes.c_size_t, P],
+    ),
+    "tread_adjust_logits": (
+        ctypes.c_int,
+        [P, I64, P, I64, ctypes.c_int, ctypes.c_int, P, I64, ctypes.c_int, P, P, P, F32, P, F32, P, F32, P, I64, P,
+         I64, ctypes.c_int, P, I64, ctypes.c_int, ctypes.c_int, P],
+    ),
     "tread_kv_fetch": (ctypes.c_int, [P, P, ctypes.c_size_t, P]),
     "tread_kv_spill": (ctypes.c_int, [P, P, ctypes.c_size_t, P]),
     "tread_kv_fetch_rows": (ctypes.c_int, [P, ctypes.c_size_t, P, ctypes.c_size_t, ctypes.c_size_t,

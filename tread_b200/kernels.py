@@ -472,6 +472,216 @@ def rows_gemm(x, w, bias=None, out=None, accumulate=False, err=None, stream=None
     return out
 
 
+# ---- decode step over a paged cache ---------------------------------------------------------------
+
+def _pages(k_pages, v_pages):
+    """(page stride, head stride) of a pair of pools [N, Hkv, page_size, D] with contiguous
+    [page_size, D] planes: a whole pool, or one layer of [N, L, Hkv, page_size, D]."""
+    C.require_cuda(k_pages, "k_pages")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+        raise ValueError("k_pages and v_pages must be [pages, Hkv, page_size, D] of one shape and strides")
+    sp, sh, st, sd = k_pages.stride()
+    if (sd != 1 and k_pages.shape[3] != 1) or st != k_pages.shape[3] or k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must share a dtype and have contiguous [page_size, D] planes")
+    return sp, sh
+
+
+def _table(table, name="table"):
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise ValueError(f"{name} must be int32 [sequences, pages] with unit column stride")
+    return table.stride(0)
+
+
+def _index(t, n, dtype, name):
+    if t.shape != (n,) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of length {n}")
+
+
+def _launch(fn, name, device, stream, *args):
+    """Call the library's fn(*args, stream) with `device` current."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _stream_arg(stream, device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream_arg(stream, device))
+    C.check(rc, name)
+
+
+def _empty(shape, dtype, device, stream):
+    """An uninitialised tensor that belongs to the stream that the launch goes to."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, rope_pos=None, attn_scaling=1.0, q=None,
+                 q_out=None, err=None, stream=None):
+    """Write the keys and values of new tokens into their pages, rotating keys and queries on the way.
+
+    k, v: [R, Hkv, D] views with unit last stride (columns of a fused projection, or a dense cache
+      [Hkv, R, D] transposed); q: [R, Hq, D] likewise, or None.
+    k_pages, v_pages: pools [pages, Hkv, page_size, D]; table: int32 [sequences, pages a sequence].
+    pos: int64 [R], each row's token position in its sequence; a negative one marks a padding row, which
+      appends nothing and whose rotated query is zero. seq: int32 [R], the row's sequence (default: row
+      r is sequence r). No two rows may name the same token.
+    inv_freq: fp32 CUDA tensor [D/2] of RoPE frequencies, or None to copy the keys (then without q).
+    rope_pos: int64 [R], the positions to rotate by where they are not `pos` (a cached block that moves
+      is re-rotated by its offset).
+    err: device error word; a row whose sequence, position or page is out of range appends nothing, gets
+      a zero query and sets bit 0.
+    Returns the rotated queries [R, Hq, D] (q_out, which may be q itself), or None without q."""
+    sp, sh = _pages(k_pages, v_pages)
+    N, Hkv, page_size, D = k_pages.shape
+    C.same_device(k_pages, k=k, v=v, v_pages=v_pages, table=table, pos=pos, seq=seq, inv_freq=inv_freq,
+                  rope_pos=rope_pos, q=q, q_out=q_out, err=err)
+    if k.dim() != 3 or k.shape[1:] != (Hkv, D) or k.stride(2) != 1 or v.shape != k.shape or v.stride(2) != 1:
+        raise ValueError(f"k and v must be [R, {Hkv}, {D}] with unit last stride")
+    R = k.shape[0]
+    if not (k.dtype == v.dtype == k_pages.dtype):
+        raise TypeError("k, v and the pages must share a dtype")
+    ld = _table(table)
+    _index(pos, R, torch.int64, "pos")
+    if seq is not None:
+        _index(seq, R, torch.int32, "seq")
+    elif R > table.shape[0]:
+        raise ValueError(f"{R} rows without seq, but a table of {table.shape[0]} sequences")
+    if rope_pos is not None:
+        _index(rope_pos, R, torch.int64, "rope_pos")
+    if inv_freq is not None:
+        _index(inv_freq, D // 2, torch.float32, "inv_freq")
+    Hq = q_ld = q_sh = 0
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out without q")
+    else:
+        if q.dim() != 3 or q.shape[0] != R or q.shape[2] != D or q.stride(2) != 1 or q.dtype != k.dtype:
+            raise ValueError(f"q must be [{R}, Hq, {D}] of k's dtype with unit last stride")
+        if inv_freq is None:
+            raise ValueError("q without inv_freq: nothing rotates it")
+        Hq, q_ld, q_sh = q.shape[1], q.stride(0), q.stride(1)
+        if q_out is None:
+            q_out = _empty(q.shape, q.dtype, q.device, stream)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
+            raise ValueError(f"q_out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
+    _launch(C.lib().tread_paged_append, "tread_paged_append", k_pages.device, stream, k.data_ptr(), k.stride(0),
+            k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _ptr(q), q_ld, q_sh, _ptr(q_out), k_pages.data_ptr(),
+            v_pages.data_ptr(), sp, sh, N, page_size, table.data_ptr(), ld, table.shape[0], table.shape[1], _ptr(seq),
+            pos.data_ptr(), _ptr(rope_pos), R, Hq, Hkv, D, _ptr(inv_freq), float(attn_scaling),
+            C.dtype_code(k.dtype), _ptr(err))
+    return q_out
+
+
+def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=None, stream=None):
+    """Attention of one new token per sequence: q [B, Hq, D] (rows at any stride) attends to the first
+    lens[b] tokens (int64 [B], the new token's own keys among them) in the pages table[b] (int32
+    [B, pages]) of the pools [pages, Hkv, page_size, D], with GQA. Where no key
+    has a score above -inf, or there is none (length 0), the output is zero.
+    err: device error word; a length that the table has no pages for gives a row of zeros and sets bit
+    1, and so does a page id outside the pool, whose keys count as masked. Returns out [B, Hq, D]."""
+    sp, sh = _pages(k_pages, v_pages)
+    N, Hkv, page_size, D = k_pages.shape
+    C.same_device(k_pages, q=q, v_pages=v_pages, table=table, lens=lens, out=out, err=err)
+    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != D) or (
+            q.dtype != k_pages.dtype):
+        raise ValueError(f"q must be [B, Hq, {D}] of the pages' dtype with contiguous rows")
+    B, Hq = q.shape[0], q.shape[1]
+    ld = _table(table)
+    if table.shape[0] != B:
+        raise ValueError(f"table must have a row for each of the {B} sequences")
+    _index(lens, B, torch.int64, "lens")
+    if out is None:
+        out = _empty(q.shape, q.dtype, q.device, stream)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
+    lib = C.lib()
+    ws = _empty((lib.tread_paged_attn_workspace_bytes(Hq, Hkv, D),), torch.uint8, q.device, stream)
+    _launch(lib.tread_paged_attn, "tread_paged_attn", q.device, stream, q.data_ptr(), q.stride(0), k_pages.data_ptr(),
+            v_pages.data_ptr(), sp, sh, N, page_size, table.data_ptr(), ld, table.shape[1], lens.data_ptr(), B, Hq, Hkv,
+            D, D ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), C.dtype_code(q.dtype), _ptr(err),
+            ws.data_ptr(), ws.numel())
+    return out
+
+
+def _per_row(x, B, name, device):
+    """A penalty as (device pointer or None, value for all rows)."""
+    if isinstance(x, torch.Tensor):
+        if x.device != device:
+            raise ValueError(f"{name} is on {x.device}, the logits on {device}")
+        _index(x, B, torch.float32, name)
+        return x.data_ptr(), 0.0
+    return None, float(x)
+
+
+def _by_row(t, B, width, dtype, name):
+    """Row stride of t [B, width], or 0 for one row [width] that serves every row."""
+    if t.dtype != dtype or t.dim() not in (1, 2) or t.shape[-1] != width or (width > 1 and t.stride(-1) != 1) or (
+            t.dim() == 2 and t.shape[0] != B):
+        raise ValueError(f"{name} must be {dtype} [{B}, {width}] or [{width}] with unit last stride")
+    return t.stride(0) if t.dim() == 2 else 0
+
+
+def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1.0, presence=0.0, frequency=0.0,
+                  bias_ids=None, bias=None, allowed=None, out=None, stream=None):
+    """The next token's logits [B, V] with penalties for repeated tokens, biases and a grammar's mask.
+
+    tokens: int64 [B, H] history (prompt, then output), the first lens[b] of it (int64 [B]; default H)
+      valid and the first prompt_lens[b] (int64 [B]; default 0) the prompt. Ids outside [0, V) count for
+      nothing.
+    repetition, presence, frequency: a number, or fp32 [B]. Per token, in this order and in fp32:
+      in the history: x / repetition where x > 0, else x * repetition;
+      x - frequency * n - presence * (n > 0), n = how often the output holds it;
+      x + its biases: bias (fp32) of bias_ids (int64), both [B, N], or [N] for all rows; several biases
+      of one token add up;
+      -inf where the grammar does not allow it: bit v % 32 of allowed[..., v // 32] (int32 [B, W], or
+      [W] for all rows, W = ceil(V / 32)) is 0.
+    Returns out: fp32 [B, V] by default; a given one may be of any supported dtype, or logits itself."""
+    C.require_cuda(logits, "logits")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [B, V] with unit column stride")
+    B, V = logits.shape
+    device = logits.device
+    C.same_device(logits, tokens=tokens, lens=lens, prompt_lens=prompt_lens, bias_ids=bias_ids, bias=bias,
+                  allowed=allowed, out=out)
+    H = tok_ld = 0
+    if tokens is not None:
+        if tokens.dim() != 2 or tokens.shape[0] != B or tokens.dtype != torch.int64 or (
+                tokens.shape[1] > 1 and tokens.stride(1) != 1):
+            raise ValueError(f"tokens must be int64 [{B}, H] with unit column stride")
+        H, tok_ld = tokens.shape[1], tokens.stride(0)
+    for t, name in ((lens, "lens"), (prompt_lens, "prompt_lens")):
+        if t is not None:
+            if tokens is None:
+                raise ValueError(f"{name} without tokens")
+            _index(t, B, torch.int64, name)
+    rep, pres, freq = (_per_row(x, B, n, device) for x, n in ((repetition, "repetition"), (presence, "presence"),
+                                                              (frequency, "frequency")))
+    if rep[0] is None and not rep[1] > 0:
+        raise ValueError(f"repetition must be above 0, got {repetition}")
+    nb = ids_ld = bias_ld = 0
+    if (bias is None) != (bias_ids is None):
+        raise ValueError("bias and bias_ids come together")
+    if bias is not None:
+        nb = bias_ids.shape[-1]
+        ids_ld, bias_ld = _by_row(bias_ids, B, nb, torch.int64, "bias_ids"), _by_row(bias, B, nb, torch.float32, "bias")
+    allowed_ld = 0 if allowed is None else _by_row(allowed, B, (V + 31) // 32, torch.int32, "allowed")
+    if out is None:
+        out = _empty((B, V), torch.float32, device, stream)
+    elif out.shape != (B, V) or (V > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be [{B}, {V}] with unit column stride")
+    elif out.data_ptr() == logits.data_ptr() and (out.dtype != logits.dtype or out.stride(0) != logits.stride(0)):
+        raise ValueError("out over logits must have their dtype and row stride")
+    _launch(C.lib().tread_adjust_logits, "tread_adjust_logits", device, stream, logits.data_ptr(), logits.stride(0),
+            out.data_ptr(), out.stride(0), B, V, _ptr(tokens), tok_ld, H, _ptr(lens), _ptr(prompt_lens),
+            rep[0], rep[1] if rep[0] is None else 1.0, pres[0], pres[1], freq[0], freq[1], _ptr(bias_ids), ids_ld,
+            _ptr(bias), bias_ld, nb, _ptr(allowed), allowed_ld, C.dtype_code(logits.dtype), C.dtype_code(out.dtype))
+    return out
+
+
 # ---- fused row-wise layer pieces ----------------------------------------------------------------
 
 def rmsnorm(x, weight, eps, out=None, stream=None):
