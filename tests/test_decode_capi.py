@@ -42,7 +42,9 @@ def _attn_call(**over):
     (dict(B=-1), "B < 0"), (dict(q=None), "null"), (dict(lens=None), "null"), (dict(Hq=3), "heads"),
     (dict(Hq=34), "heads"), (dict(Hkv=0), "heads"), (dict(D=96), "head_dim"), (dict(dtype=9), "dtype"),
     (dict(page=0), "page geometry"), (dict(hs=16), "page geometry"), (dict(table=None), "page table"),
-    (dict(t_ld=2), "page table"),
+    (dict(t_ld=2), "page table"), (dict(q=264), "16-byte"), (dict(kp=264), "16-byte"), (dict(out=264), "16-byte"),
+    (dict(q_ld=516), "16-byte"), (dict(ps=2 * 16 * 128 + 4), "16-byte"), (dict(P=2 ** 28, t_ld=2 ** 28), "2^31"),
+    (dict(ws=None), "workspace"), (dict(ws=264), "workspace"), (dict(ws_bytes=100), "workspace"),
 ])
 def test_paged_attn_rejects_bad_arguments(over, needle):
     assert _attn_call(**over) == 1

@@ -167,17 +167,6 @@ def test_shared_pages_and_repeated_calls_give_the_same_bits():
         assert torch.equal(kernels.paged_attn(q, kp, vp, table, lens), got)
 
 
-def test_unaligned_pools():
-    """Pools that start 2 bytes off a 16-byte boundary."""
-    c = q, kp, vp, table, lens = _case([100, 33], 4, 2, 64, 16, BF, 10)
-    moved = []
-    for p in (kp, vp):
-        flat = torch.empty(p.numel() + 1, dtype=BF, device=DEV)
-        flat[1:] = p.flatten()
-        moved.append(flat[1:].view(p.shape))
-    _check(kernels.paged_attn(q, *moved, table, lens), *c)
-
-
 def test_other_streams_and_graphs():
     """Two graphs with calls of different sizes, and an eager call, each on a stream of its own, replayed
     together again and again."""
@@ -238,5 +227,10 @@ def test_attn_refuses_bad_tensors():
             kernels.paged_attn(**{**dict(q=q, k_pages=kp, v_pages=vp, table=table, lens=lens), **bad})
     with pytest.raises(RuntimeError, match="heads"):
         kernels.paged_attn(q[:, :3], kp, vp, table, lens)
+    off = torch.empty(kp.numel() + 1, dtype=BF, device=DEV)[1:].view(kp.shape)  # 2 bytes off a 16-byte boundary
+    with pytest.raises(RuntimeError, match="16-byte"):
+        kernels.paged_attn(q, off, vp, table, lens)
+    with pytest.raises(RuntimeError, match="16-byte"):
+        kernels.paged_attn(torch.empty(2, 4 * 64 + 1, dtype=BF, device=DEV)[:, :256].unflatten(1, (4, 64)), kp, vp, table, lens)
     with pytest.raises(RuntimeError, match="head_dim"):
         kernels.paged_attn(q[..., :32].contiguous(), kp[..., :32].contiguous(), vp[..., :32].contiguous(), table, lens)

@@ -3,12 +3,36 @@
 //   out[b, h] = sum_t softmax_t(scale * q[b, h] . K[t, g]) V[t, g],   t < lens[b], g = h / (Hq / Hkv)
 // where token t's keys and values lie in slot t % page_size of page table[b][t / page_size]. Where no
 // key has a score above -inf, or there is none, the softmax has no value and the output is zero.
+//
+// Every key and value is read once: 4 D bytes a token and KV head in 16 bits, against 4 D G operations
+// (G = Hq / Hkv query heads share them). At G = 7 that is 7 operations a byte, far below what the tensor
+// cores need to be busy: the bound is HBM, and for few keys the latency of a launch.
+//
+// Split. The lengths are on the device, so the kernel itself deals out the work: all sequences' keys, per
+// KV head in units of 16, form one line that is cut into equal shares, one per CTA, whatever the lengths.
+// A CTA's share covers parts of one or more items (sequence, KV head). Its warps take the units of the
+// share in turn, each with a ring of units in flight in shared memory (cp.async, 16 bytes a lane, rows
+// swizzled so that eight rows' same chunk lie in eight banks), its own running maximum and sum, and its
+// own accumulators. At an item's end the warps' states are joined in shared memory; an item that several
+// CTAs share leaves its states in the workspace, where a second kernel joins them in the order of the
+// shares (no atomics: the result does not depend on timing).
+//
+// 16-bit types run on mma.sync with keys as rows and the group's query heads as the 8 columns, so that a
+// group of 7 fills 7 of 8 columns (heads as rows would fill 7 of 16): S^T = K Q^T, O^T = V^T P^T, and the
+// heads of S^T's, P^T's and O^T's columns stay in the same lanes. P is rounded to the type once before it
+// meets V (its sum stays fp32): half a step of each weight, the size of the output's own rounding.
+// fp32 runs on FMAs.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace tread {
 namespace {
 
-constexpr int kTile = 32;
+constexpr int kUnit = 16;      // keys of one unit
+constexpr int kMaxCtas = 384;  // shares at most
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.f;  // the running maximum may lag by 2^8: weights stay far inside fp16's range
 
 struct DecodeArgs {
   const void* q;
@@ -18,119 +42,646 @@ struct DecodeArgs {
   long long q_ld, page_stride, head_stride, num_pages, table_ld;
   const int32_t* table;
   const int64_t* lens;
-  int B, Hq, Hkv, max_pages, page_size;
-  float scale;
+  int B, Hq, Hkv, G, max_pages, page_size;
+  float scale_log2;
   unsigned* err;
+  int4* desc;   // [kMaxCtas] {parts of the item that starts in this CTA and ends in another, b, g, slot}
+  float2* ml;   // [kMaxCtas][2][G] {maximum, sum} of the partial states
+  float* part;  // [kMaxCtas][2][G][D]
 };
 
-// The simplest form: one CTA per (sequence, KV head), one warp per query head of the group, 32 keys at a
-// time through shared memory.
-template <typename T, int D>
-__global__ void paged_attn_kernel(const __grid_constant__ DecodeArgs a) {
-  constexpr int DPL = D / 32;
-  extern __shared__ float smem[];
-  const int G = a.Hq / a.Hkv;
-  float* qs = smem;                  // [G][D]
-  float* ks = qs + G * D;            // [kTile][D + 1]
-  float* vs = ks + kTile * (D + 1);  // [kTile][D]
-  __shared__ long long s_row[kTile];
-  const int b = blockIdx.x, g = blockIdx.y;
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  long long n = a.lens[b];
-  if (n < 0 || n > (long long)a.max_pages * a.page_size) {
-    if (threadIdx.x == 0 && a.err) atomicOr(a.err, 2u);
-    n = 0;
-  }
-  for (int i = threadIdx.x; i < G * D; i += blockDim.x)
-    qs[i] = Num<T>::to_f(static_cast<const T*>(a.q)[b * a.q_ld + (long long)g * G * D + i]);
-  float m = -INFINITY, l = 0.f, o[DPL];
-#pragma unroll
-  for (int k = 0; k < DPL; ++k) o[k] = 0.f;
-  for (long long t0 = 0; t0 < n; t0 += kTile) {
-    const int nt = (int)(n - t0 < kTile ? n - t0 : kTile);
-    __syncthreads();
-    if (threadIdx.x < kTile) {
-      long long row = -1;
-      if (threadIdx.x < nt) {
-        const long long t = t0 + threadIdx.x, pg = t / a.page_size;
-        const int id = a.table[b * a.table_ld + pg];
-        if (id >= 0 && id < a.num_pages)
-          row = id * a.page_stride + g * a.head_stride + (t - pg * a.page_size) * D;
-        else if (a.err)
-          atomicOr(a.err, 2u);
-      }
-      s_row[threadIdx.x] = row;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTile * D; i += blockDim.x) {
-      const int j = i / D, d = i - j * D;
-      float kv = 0.f, vv = 0.f;
-      if (s_row[j] >= 0) {
-        kv = Num<T>::to_f(static_cast<const T*>(a.k_pages)[s_row[j] + d]);
-        vv = Num<T>::to_f(static_cast<const T*>(a.v_pages)[s_row[j] + d]);
-      }
-      ks[j * (D + 1) + d] = kv;
-      vs[j * D + d] = vv;
-    }
-    __syncthreads();
-    float s = -INFINITY;
-    if (s_row[lane] >= 0) {
-      float acc = 0.f;
-#pragma unroll 8
-      for (int d = 0; d < D; ++d) acc = fmaf(qs[w * D + d], ks[lane * (D + 1) + d], acc);
-      s = acc * a.scale;
-    }
-    float top = s;
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float m_new = fmaxf(m, top);
-    if (m_new == -INFINITY) continue;  // no key so far
-    const float p = s_row[lane] >= 0 ? expf(s - m_new) : 0.f;
-    const float alpha = expf(m - m_new);
-    float sum = p;
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    l = l * alpha + sum;
-#pragma unroll
-    for (int k = 0; k < DPL; ++k) o[k] *= alpha;
-    for (int j = 0; j < kTile; ++j) {
-      const float pj = __shfl_sync(0xffffffffu, p, j);
-#pragma unroll
-      for (int k = 0; k < DPL; ++k) o[k] = fmaf(pj, vs[j * D + lane + 32 * k], o[k]);
-    }
-    m = m_new;
-  }
-  T* row = static_cast<T*>(a.out) + ((long long)b * a.Hq + g * G + w) * D;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int k = 0; k < DPL; ++k) row[lane + 32 * k] = Num<T>::from_f(o[k] * inv);
+__device__ __forceinline__ unsigned smem_addr(const void* p) {
+  return static_cast<unsigned>(__cvta_generic_to_shared(p));
 }
 
+__device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool read) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_x4(unsigned (&r)[4], unsigned addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(unsigned (&r)[4], unsigned addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ unsigned transpose8x8(unsigned x) {
+  unsigned y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], const unsigned (&b)[2]) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+template <typename T>
+__device__ __forceinline__ unsigned pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+  }
+}
+
+// exp2(x - m) where m may still be -inf (no finite score so far): then x is -inf too, or a NaN to pass on
+__device__ __forceinline__ float weight(float x, float m) { return exp2f(x - (m == -INFINITY ? 0.f : m)); }
+
+// Place of element d of head h in a warp's accumulators: the four head pairs of a fragment's lanes lie in
+// four groups of banks.
+template <int D>
+__device__ __forceinline__ int place_of(int h, int d) {
+  return h * D + (d ^ (((h >> 1) & 3) << 3));
+}
+
+// Shared memory and launch shape of one instance. Two CTAs per SM where their rings fit beside each
+// other, so that one joins while the other streams; about 190 KB of units in flight per SM either way.
+template <typename T, int D, int GP>
+struct Shape {
+  static constexpr int kRow = D * sizeof(T);               // bytes of one key
+  static constexpr int kUnitBytes = 2 * kUnit * kRow;      // keys, then values
+  static constexpr int kWarps = kUnitBytes > 16384 ? 2 : 4;
+  static constexpr int kJoin = kWarps * GP * D * 4;        // the warps' accumulators at an item's end
+  static constexpr int kQ = sizeof(T) == 4 ? GP * D * 4 + kWarps * kUnit * GP * 4 : 0;  // fp32: queries and weights
+  static constexpr int kCtas = kUnitBytes <= 8192 && kJoin <= 16384 ? 2 : 1;
+  static constexpr int kRoom = (kCtas == 2 ? 112 : 224) * 1024 - kJoin - kQ;
+  static constexpr int kFit = kRoom / (kWarps * kUnitBytes);
+  static constexpr int kStages = kFit > 6 ? 6 : kFit;
+  static constexpr int kSmem = kStages * kWarps * kUnitBytes + kJoin + kQ;
+  static_assert(kStages >= 2, "ring");
+};
+
+// One warp's state over 16-bit keys.
+template <typename T, int D, int GP>
+struct MmaState {
+  static constexpr int NT = GP / 8;
+  unsigned qf[NT][D / 16][2];
+  float o[NT][D / 16][4];
+  float m[NT][2], l[NT][2];  // of heads 8 nt + 2 (lane % 4) + {0, 1}; l: this lane's keys only
+
+  __device__ void start(const DecodeArgs& a, int b, int g, void*, int, int lane) {
+    const T* q = static_cast<const T*>(a.q) + b * a.q_ld + (long long)g * a.G * D;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 8 + (lane >> 2);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const unsigned* p = reinterpret_cast<const unsigned*>(q + h * D + ks * 16 + (lane & 3) * 2);
+        qf[nt][ks][0] = h < a.G ? p[0] : 0u;
+        qf[nt][ks][1] = h < a.G ? p[4] : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) m[nt][i] = -INFINITY, l[nt][i] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
+    }
+  }
+
+  __device__ __forceinline__ void unit(const DecodeArgs& a, unsigned keys, unsigned values, unsigned live, void*,
+                                       int, int lane) {
+    constexpr int kRow = D * sizeof(T);
+    float s[NT][2][4];  // two chains each, so that a product does not wait for the last one's sum
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][0][i] = s[nt][1][i] = 0.f;
+    {
+      const int row = lane & 15;
+      const unsigned base = keys + row * kRow;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        unsigned f[4];
+        ldmatrix_x4(f, base + (((2 * ks + (lane >> 4)) ^ (row & 7)) << 4));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[nt][ks & 1], f, qf[nt][ks]);
+      }
+    }
+    const bool live0 = (live >> (lane >> 2)) & 1, live1 = (live >> ((lane >> 2) + 8)) & 1;
+    unsigned p[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (s[nt][0][i] + s[nt][1][i]) * a.scale_log2;
+      if (live != 0xffffu) {
+        if (!live0) x[0] = x[1] = -INFINITY;
+        if (!live1) x[2] = x[3] = -INFINITY;
+      }
+      float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+      // the maximum moves only when a score leaves it behind by more than kSlack: rarely
+      if (__any_sync(0xffffffffu, top[0] > m[nt][0] + kSlack || top[1] > m[nt][1] + kSlack)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+          const float next = fmaxf(m[nt][i], top[i]);
+          const float alpha = weight(m[nt][i], next);
+          m[nt][i] = next;
+          l[nt][i] *= alpha;
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt) o[nt][mt][i] *= alpha, o[nt][mt][i + 2] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = weight(x[i], m[nt][i & 1]);
+      l[nt][0] += x[0] + x[2];
+      l[nt][1] += x[1] + x[3];
+      p[nt][0] = transpose8x8(pack2<T>(x[0], x[1]));
+      p[nt][1] = transpose8x8(pack2<T>(x[2], x[3]));
+    }
+    {
+      const int row = (lane & 7) + ((lane >> 4) << 3);
+      const unsigned base = values + row * kRow;
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt) {
+        unsigned f[4];
+        ldmatrix_x4_trans(f, base + (((2 * mt + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][mt], f, p[nt]);
+      }
+    }
+  }
+
+  // the state into shared memory: accumulators [GP][D] (place_of), maxima and sums [GP]
+  __device__ void leave(float* so, float2* sml, int lane) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float sum = l[nt][i];
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        const int h = nt * 8 + (lane & 3) * 2 + i;
+        if (lane < 4) sml[h] = make_float2(m[nt][i], sum);
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) {
+          so[place_of<D>(h, mt * 16 + (lane >> 2))] = o[nt][mt][i];
+          so[place_of<D>(h, mt * 16 + (lane >> 2) + 8)] = o[nt][mt][i + 2];
+        }
+      }
+    }
+  }
+};
+
+// One warp's state over fp32 keys: scores with a half warp per half of D and a lane per key, then values
+// with D / 32 elements a lane.
+template <int D, int GP>
+struct FmaState {
+  static constexpr int kPer = D / 32;
+  float o[GP][kPer], m[GP], l[GP];  // l: this lane's key only
+
+  __device__ void start(const DecodeArgs& a, int b, int g, void* extra, int warp, int lane) {
+    float* sq = static_cast<float*>(extra);
+    const float* q = static_cast<const float*>(a.q) + b * a.q_ld + (long long)g * a.G * D;
+    for (int i = threadIdx.x; i < GP * D; i += blockDim.x) sq[i] = i < a.G * D ? q[i] : 0.f;
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      m[h] = -INFINITY, l[h] = 0.f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[h][e] = 0.f;
+    }
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void unit(const DecodeArgs& a, unsigned keys, unsigned values, unsigned live, void* extra,
+                                       int warp, int lane) {
+    constexpr int kRow = D * 4;
+    const float* sq = static_cast<const float*>(extra);
+    float* sp = static_cast<float*>(extra) + GP * D + warp * kUnit * GP;  // [kUnit][GP]
+    const int key = lane & 15, half = lane >> 4;
+    float s[GP];
+#pragma unroll
+    for (int h = 0; h < GP; ++h) s[h] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < D / 8; ++i) {
+      const int c = half * (D / 8) + i;
+      float4 k;
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(k.x), "=f"(k.y), "=f"(k.z), "=f"(k.w)
+                   : "r"(keys + key * kRow + ((c ^ (key & 7)) << 4))
+                   : "memory");
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        const float4 q = *reinterpret_cast<const float4*>(sq + h * D + c * 4);
+        s[h] = fmaf(k.x, q.x, s[h]);
+        s[h] = fmaf(k.y, q.y, s[h]);
+        s[h] = fmaf(k.z, q.z, s[h]);
+        s[h] = fmaf(k.w, q.w, s[h]);
+      }
+    }
+    const bool on = (live >> key) & 1;
+    bool moved = false;
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      s[h] = (s[h] + __shfl_xor_sync(0xffffffffu, s[h], 16)) * a.scale_log2;
+      if (!on) s[h] = -INFINITY;
+      moved |= s[h] > m[h] + kSlack;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        float top = s[h];
+#pragma unroll
+        for (int off = 1; off <= 8; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float next = fmaxf(m[h], top);
+        const float alpha = weight(m[h], next);
+        m[h] = next;
+        l[h] *= alpha;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) o[h][e] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      s[h] = weight(s[h], m[h]);
+      if (half == 0) {
+        l[h] += s[h];
+        sp[key * GP + h] = s[h];
+      }
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int t = 0; t < kUnit; ++t) {
+      float v[kPer];
+      if constexpr (kPer == 2) {
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(v[0]), "=f"(v[1])
+                     : "r"(values + t * kRow + (((lane >> 1) ^ (t & 7)) << 4) + (lane & 1) * 8)
+                     : "memory");
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; e += 4)
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[e]), "=f"(v[e + 1]), "=f"(v[e + 2]), "=f"(v[e + 3])
+                       : "r"(values + t * kRow + (((lane + e * 8) ^ (t & 7)) << 4))
+                       : "memory");
+      }
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        const float w = sp[t * GP + h];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) o[h][e] = fmaf(w, v[e], o[h][e]);
+      }
+    }
+    __syncwarp();  // the weights are written again by the next unit
+  }
+
+  __device__ void leave(float* so, float2* sml, int lane) {
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      float sum = l[h];
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (lane == 0) sml[h] = make_float2(m[h], sum);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        so[place_of<D>(h, kPer == 2 ? lane * 2 + e : (e / 4) * 128 + lane * 4 + e % 4)] = o[h][e];
+    }
+  }
+};
+
+template <typename T, int D, int GP>
+struct StateOf {
+  using type = MmaState<T, D, GP>;
+};
+template <int D, int GP>
+struct StateOf<float, D, GP> {
+  using type = FmaState<D, GP>;
+};
+
+// A sequence's length, 0 where it is out of range.
+__device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
+  const long long n = __ldg(reinterpret_cast<const long long*>(a.lens) + b);
+  return n < 0 || n > (long long)a.max_pages * a.page_size ? 0 : (int)n;
+}
+__device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kUnit; }
+
+// A place on the line of units: unit j of item (b, g), the item having n units of len tokens.
+struct Place {
+  int b, g, j, n, len;
+
+  __device__ __forceinline__ void settle(const DecodeArgs& a) {  // j may lie behind the item's end
+    while (j >= n) {
+      j -= n;
+      if (++g < a.Hkv) continue;
+      g = 0;
+      do {
+        if (++b >= a.B) {
+          n = 1 << 30, j = 0, b = a.B - 1, len = 0;  // the line's end: never loaded
+          return;
+        }
+        len = length_of(a, b);
+        n = units_of(len);
+      } while (n == 0);
+    }
+  }
+};
+
+template <typename T, int D, int GP, bool WHOLE>  // WHOLE: a unit never crosses a page (page_size % 16 == 0)
+__global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
+    paged_attn_kernel(const __grid_constant__ DecodeArgs a) {
+  using S = Shape<T, D, GP>;
+  constexpr int W = S::kWarps, kThreads = W * 32, kStages = S::kStages;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ unsigned s_live[W][kStages];
+  __shared__ float2 s_ml[W][GP];
+  __shared__ long long s_scan[kThreads / 32];
+  __shared__ Place s_place;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* s_o = reinterpret_cast<float*>(smem + kStages * W * S::kUnitBytes);
+  void* extra = smem + kStages * W * S::kUnitBytes + S::kJoin;
+  const unsigned ring = smem_addr(smem) + warp * (kStages * S::kUnitBytes);
+
+  // the line: every thread adds up a run of sequences, a scan places the runs
+  const int run = (a.B + kThreads - 1) / kThreads;
+  const int b0 = min(a.B, (int)threadIdx.x * run), b1 = min(a.B, b0 + run);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int len = length_of(a, b);
+    mine += units_of(len);
+    if (len == 0 && b % gridDim.x == blockIdx.x) {
+      const long long n = __ldg(reinterpret_cast<const long long*>(a.lens) + b);
+      if (n != 0 && a.err) atomicOr(a.err, 2u);
+    }
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += x;
+  }
+  if (lane == 31) s_scan[warp] = upto;
+  if (threadIdx.x == 0) s_place.b = -1;
+  __syncthreads();
+  long long before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
+  total *= a.Hkv;
+  long long share = (total + gridDim.x - 1) / gridDim.x;
+  if (share < W) share = W;  // a unit for every warp at least: more parts cost more to join
+  const long long u0 = blockIdx.x * share, u1 = min(total, u0 + share);
+  if (u0 < u1 && u0 >= before * a.Hkv && u0 < (before + mine) * a.Hkv) {
+    long long at = before * a.Hkv;
+    for (int b = b0;; ++b) {
+      const int len = length_of(a, b), n = units_of(len);
+      if (u0 < at + (long long)n * a.Hkv) {
+        const int in = (int)(u0 - at);
+        s_place = Place{b, in / n, in % n, n, len};
+        break;
+      }
+      at += (long long)n * a.Hkv;
+    }
+  }
+  // sequences without a key: zeros
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (length_of(a, b) == 0)
+      for (int i = threadIdx.x; i < a.Hq * D; i += kThreads)
+        static_cast<T*>(a.out)[(long long)b * a.Hq * D + i] = Num<T>::from_f(0.f);
+  __syncthreads();
+  if (u0 >= u1) {
+    if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
+
+  // the warp's own walk along the share, kStages - 1 units ahead of what it computes
+  Place load = s_place;
+  load.j += warp;
+  load.settle(a);
+  long long load_at = u0 + warp;
+  auto page_of = [&]() -> int {  // of the unit's first key, or of the lane's key
+    const unsigned t = load.j * kUnit + (WHOLE ? 0 : lane & 15);
+    return load_at < u1 && t < (unsigned)load.len ? __ldg(a.table + load.b * a.table_ld + t / (unsigned)a.page_size)
+                                                  : -1;
+  };
+  int id = page_of();
+  auto fetch = [&](int stage) {
+    if (load_at < u1) {
+      constexpr int kChunks = S::kRow / 16, kIter = kUnit * kChunks / 32;
+      const unsigned dst = ring + stage * S::kUnitBytes;
+      const unsigned t0 = load.j * kUnit, t = t0 + (WHOLE ? 0 : lane & 15);
+      const bool known = id >= 0 && id < a.num_pages;
+      const unsigned slot = t - t / (unsigned)a.page_size * a.page_size;
+      const long long off = known ? id * a.page_stride + load.g * a.head_stride + (long long)slot * D : 0;
+      const int rows = min(kUnit, load.len - (int)t0);
+      unsigned live = (1u << rows) - 1;
+      if (WHOLE) {
+        if (!known) live = 0;
+      } else {
+        live &= __ballot_sync(0xffffffffu, known);  // lanes 16..31 repeat lanes 0..15
+      }
+      if (live != (1u << rows) - 1 && lane == 0 && a.err) atomicOr(a.err, 2u);
+      if (lane == 0) s_live[warp][stage] = live;
+      const char* kp = static_cast<const char*>(a.k_pages);
+      const char* vp = static_cast<const char*>(a.v_pages);
+#pragma unroll
+      for (int it = 0; it < kIter; ++it) {
+        const int row = (it * 32 + lane) / kChunks, c = (it * 32 + lane) % kChunks;
+        long long from;
+        if constexpr (WHOLE)
+          from = (off + (long long)row * D) * (int)sizeof(T) + c * 16;
+        else
+          from = __shfl_sync(0xffffffffu, off, row) * (int)sizeof(T) + c * 16;
+        const bool read = (live >> row) & 1;
+        const unsigned to = dst + row * S::kRow + ((c ^ (row & 7)) << 4);
+        cp_async16(to, kp + (read ? from : 0), read);  // rows that are not read are zero
+        cp_async16(to + kUnit * S::kRow, vp + (read ? from : 0), read);
+      }
+      load_at += W;
+      load.j += W;
+      load.settle(a);
+      id = page_of();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+
+  Place at = s_place;
+  long long pos = u0;
+  int step = 0;  // the warp's units so far, modulo the ring
+  int4 open = make_int4(0, 0, 0, 0);
+  typename StateOf<T, D, GP>::type st;
+  while (pos < u1) {
+    const int seg = (int)min((long long)(at.n - at.j), u1 - pos);
+    st.start(a, at.b, at.g, extra, warp, lane);
+    const int skip = (int)((pos - u0) % W);
+    for (int i = warp >= skip ? warp - skip : warp - skip + W; i < seg; i += W) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      const unsigned stage = ring + step * S::kUnitBytes;
+      const unsigned live = s_live[warp][step];
+      fetch(step == 0 ? kStages - 1 : step - 1);  // into the place of the unit before, which every lane has read
+      st.unit(a, stage, stage + kUnit * S::kRow, live, extra, warp, lane);
+      step = step + 1 == kStages ? 0 : step + 1;
+    }
+    // the item's end, or the share's: join the warps
+    st.leave(s_o + warp * GP * D, s_ml[warp], lane);
+    __syncthreads();
+    const bool whole = seg == at.n;
+    const int slot = pos == u0 ? 0 : 1;
+    const long long p = (long long)blockIdx.x * 2 + slot;
+    for (int i = threadIdx.x; i < a.G * (D / 2); i += kThreads) {
+      const int h = i / (D / 2), d = i % (D / 2) * 2;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][h].x);
+      float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = weight(s_ml[w][h].x, top);
+        const float2 o = *reinterpret_cast<const float2*>(s_o + w * GP * D + place_of<D>(h, d));
+        sum += f * s_ml[w][h].y;
+        x += f * o.x;
+        y += f * o.y;
+      }
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T* to = static_cast<T*>(a.out) + ((long long)at.b * a.Hq + at.g * a.G + h) * D + d;
+        to[0] = Num<T>::from_f(x * inv);
+        to[1] = Num<T>::from_f(y * inv);
+      } else {
+        *reinterpret_cast<float2*>(a.part + (p * a.G + h) * D + d) = make_float2(x, y);
+        if (d == 0) a.ml[p * a.G + h] = make_float2(top, sum);
+      }
+    }
+    if (!whole && at.j == 0)  // starts here, ends in the CTA of its last unit
+      open = make_int4((int)((pos + at.n - 1) / share - blockIdx.x + 1), at.b, at.g, slot);
+    pos += seg;
+    at.j += seg;
+    if (pos < u1) at.settle(a);
+    __syncthreads();
+  }
+  cp_async_wait<0>();
+  if (threadIdx.x == 0) a.desc[blockIdx.x] = open;
+}
+
+// Items whose keys several CTAs share: CTA (c, h) joins head h of the item that starts in share c and
+// ends in another. Its four warps take the parts in turn.
+constexpr int kJoinWarps = 4;
+
 template <typename T, int D>
-int launch(const DecodeArgs& a, cudaStream_t st) {
-  const int G = a.Hq / a.Hkv;
-  const int smem = (int)sizeof(float) * (G * D + kTile * (D + 1) + kTile * D);
-  auto kern = paged_attn_kernel<T, D>;
-  if (smem > 48 * 1024 - 512)
-    TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kern<<<dim3(a.B, a.Hkv), 32 * G, smem, st>>>(a);
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const __grid_constant__ DecodeArgs a) {
+  constexpr int kPer = D / 32;
+  __shared__ float s_o[kJoinWarps][D], s_l[kJoinWarps], s_m[kJoinWarps];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 open = a.desc[blockIdx.x];
+  if (open.x == 0) return;
+  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto state = [&](int i) { return ((blockIdx.x + i) * 2LL + (i == 0 ? open.w : 0)) * a.G + h; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < open.x; i += kJoinWarps * 32) top = fmaxf(top, a.ml[state(i)].x);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  if (lane == 0) s_m[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_m[w]);
+  float sum = 0.f, o[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < open.x; i += kJoinWarps) {
+    const float2 ml = a.ml[state(i)];
+    const float* from = a.part + state(i) * D + lane * kPer;
+    float x[kPer];
+    if constexpr (kPer == 2) {
+      *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(x + e) = *reinterpret_cast<const float4*>(from + e);
+    }
+    const float f = weight(ml.x, top);
+    sum += f * ml.y;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] = fmaf(f, x[e], o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) s_o[warp][lane * kPer + e] = o[e];
+  if (lane == 0) s_l[warp] = sum;
+  __syncthreads();
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) all += s_l[w];
+  const float inv = all == 0.f ? 0.f : 1.f / all;
+  T* to = static_cast<T*>(a.out) + ((long long)open.y * a.Hq + open.z * a.G + h) * D;
+  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) x += s_o[w][d];
+    to[d] = Num<T>::from_f(x * inv);
+  }
+}
+
+template <typename T, int D, int GP>
+int launch(const DecodeArgs& a, int sms, cudaStream_t st) {
+  using S = Shape<T, D, GP>;
+  auto kern = a.page_size % kUnit == 0 ? paged_attn_kernel<T, D, GP, true> : paged_attn_kernel<T, D, GP, false>;
+  TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  int ctas = sms * S::kCtas;
+  if (ctas > kMaxCtas) ctas = kMaxCtas;
+  kern<<<ctas, S::kWarps * 32, S::kSmem, st>>>(a);
   TREAD_CHECK_LAUNCH("paged_attn_kernel");
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas, a.G);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TREAD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T, D>, a));
   return TREAD_OK;
 }
 
 template <typename T>
-int dispatch(int D, const DecodeArgs& a, cudaStream_t st) {
+int dispatch(int D, const DecodeArgs& a, int sms, cudaStream_t st) {
+  const bool few = a.G <= 8;
   switch (D) {
-    case 64: return launch<T, 64>(a, st);
-    case 128: return launch<T, 128>(a, st);
-    default: return launch<T, 256>(a, st);
+    case 64: return few ? launch<T, 64, 8>(a, sms, st) : launch<T, 64, 16>(a, sms, st);
+    case 128: return few ? launch<T, 128, 8>(a, sms, st) : launch<T, 128, 16>(a, sms, st);
+    default: return few ? launch<T, 256, 8>(a, sms, st) : launch<T, 256, 16>(a, sms, st);
   }
 }
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
 }  // namespace
 }  // namespace tread
 
-extern "C" size_t tread_paged_attn_workspace_bytes(int Hq, int Hkv, int D) { return 0; }
+extern "C" size_t tread_paged_attn_workspace_bytes(int Hq, int Hkv, int D) {
+  using namespace tread;
+  if (Hq <= 0 || Hkv <= 0 || D <= 0 || Hq / Hkv > 16 || D > 256) return 0;
+  const size_t states = (size_t)kMaxCtas * 2 * (Hq / Hkv);
+  return align256(kMaxCtas * sizeof(int4)) + align256(states * sizeof(float2)) + states * D * sizeof(float);
+}
 
 extern "C" int tread_paged_attn(const void* q, int64_t q_ld, const void* k_pages, const void* v_pages,
                                 int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
@@ -144,22 +695,40 @@ extern "C" int tread_paged_attn(const void* q, int64_t q_ld, const void* k_pages
   TREAD_CHECK_ARG(Hq > 0 && Hkv > 0 && Hkv <= 65535 && Hq % Hkv == 0 && Hq / Hkv <= 16,
                   "paged_attn: bad heads Hq=%d Hkv=%d", Hq, Hkv);
   TREAD_CHECK_ARG(D == 64 || D == 128 || D == 256, "paged_attn: head_dim %d not in {64,128,256}", D);
-  TREAD_CHECK_ARG(dtype_size(dtype) != 0, "paged_attn: unknown dtype %d", dtype);
+  const int64_t es = (int64_t)dtype_size(dtype);
+  TREAD_CHECK_ARG(es != 0, "paged_attn: unknown dtype %d", dtype);
   TREAD_CHECK_ARG(page_size > 0 && num_pages >= 0 && num_pages <= INT32_MAX &&
                       (num_pages <= 1 || page_stride >= (int64_t)page_size * D) &&
                       (Hkv == 1 || head_stride >= (int64_t)page_size * D),
                   "paged_attn: bad page geometry");
   TREAD_CHECK_ARG(max_pages >= 0 && (table || max_pages == 0) && (B <= 1 || table_ld >= max_pages),
                   "paged_attn: bad page table");
+  TREAD_CHECK_ARG((int64_t)max_pages * page_size <= INT32_MAX - kUnit, "paged_attn: a sequence of 2^31 tokens or more");
+  TREAD_CHECK_ARG(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) &&
+                      ((q_ld | page_stride | head_stride) * es) % 16 == 0,
+                  "paged_attn: q, out and pages must lie on 16-byte boundaries");
+  TREAD_CHECK_ARG(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
+                      workspace_bytes >= tread_paged_attn_workspace_bytes(Hq, Hkv, D),
+                  "paged_attn: workspace too small or not 256-byte aligned");
+  int device = 0, sms = 0;
+  TREAD_CHECK_CUDA(cudaGetDevice(&device));
+  TREAD_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
   DecodeArgs a;
   a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_ld = q_ld, a.page_stride = page_stride;
   a.head_stride = head_stride, a.num_pages = num_pages, a.table_ld = table_ld, a.table = table, a.lens = lens;
-  a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.max_pages = max_pages, a.page_size = page_size, a.scale = sm_scale;
+  a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.max_pages = max_pages, a.page_size = page_size;
+  a.scale_log2 = sm_scale * kLog2e;
   a.err = static_cast<unsigned*>(err_flag);
+  char* ws = static_cast<char*>(workspace);
+  a.desc = reinterpret_cast<int4*>(ws);
+  ws += align256(kMaxCtas * sizeof(int4));
+  a.ml = reinterpret_cast<float2*>(ws);
+  ws += align256((size_t)kMaxCtas * 2 * a.G * sizeof(float2));
+  a.part = reinterpret_cast<float*>(ws);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case TREAD_BF16: return dispatch<__nv_bfloat16>(D, a, st);
-    case TREAD_F16: return dispatch<__half>(D, a, st);
-    default: return dispatch<float>(D, a, st);
+    case TREAD_BF16: return dispatch<__nv_bfloat16>(D, a, sms, st);
+    case TREAD_F16: return dispatch<__half>(D, a, sms, st);
+    default: return dispatch<float>(D, a, sms, st);
   }
 }
