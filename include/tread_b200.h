@@ -274,14 +274,20 @@ int tread_rows_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
  *             rope_pos * inv_freq in 64 bits; cos and sin times attn_scaling in fp32; rounded once.
  * A row whose sequence, position or page id is out of range appends nothing, gets a q_out row of zeros
  * and sets bit 0 of *err_flag (may be NULL). No two rows may name the same token; D even, at most 256.
+ * The arguments of this and the next two entry points come in a struct, read during the call only.
  */
-int tread_paged_append(const void* k, int64_t k_ld, int64_t k_sh, const void* v, int64_t v_ld, int64_t v_sh,
-                       const void* q, int64_t q_ld, int64_t q_sh, void* q_out, void* k_pages, void* v_pages,
-                       int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
-                       const int32_t* table, int64_t table_ld, int num_seqs, int max_pages,
-                       const int32_t* seq, const int64_t* pos, const int64_t* rope_pos, int R, int Hq,
-                       int Hkv, int D, const float* inv_freq, float attn_scaling, int dtype,
-                       void* err_flag, tread_stream_t stream);
+typedef struct {
+  const void *k, *v, *q;
+  void *q_out, *k_pages, *v_pages;
+  const int32_t *table, *seq;
+  const int64_t *pos, *rope_pos;
+  const float* inv_freq;
+  void* err_flag;
+  int64_t k_ld, k_sh, v_ld, v_sh, q_ld, q_sh, page_stride, head_stride, num_pages, table_ld;
+  int32_t page_size, num_seqs, max_pages, R, Hq, Hkv, D, dtype;
+  float attn_scaling;
+} tread_paged_append_args;
+int tread_paged_append(const tread_paged_append_args* args, tread_stream_t stream);
 
 /*
  * Attention of one new token per sequence over its pages (the attention of tread/server.py:207-209's
@@ -299,11 +305,17 @@ int tread_paged_append(const void* k, int64_t k_ld, int64_t k_sh, const void* v,
  * irrelevant; calls that share one must be stream-ordered.
  */
 size_t tread_paged_attn_workspace_bytes(int Hq, int Hkv, int D);
-int tread_paged_attn(const void* q, int64_t q_ld, const void* k_pages, const void* v_pages,
-                     int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
-                     const int32_t* table, int64_t table_ld, int max_pages, const int64_t* lens, int B,
-                     int Hq, int Hkv, int D, float sm_scale, void* out, int dtype, void* err_flag,
-                     void* workspace, size_t workspace_bytes, tread_stream_t stream);
+typedef struct {
+  const void *q, *k_pages, *v_pages;
+  void* out;
+  const int32_t* table;
+  const int64_t* lens;
+  void *err_flag, *workspace;
+  int64_t q_ld, page_stride, head_stride, num_pages, table_ld, workspace_bytes;
+  int32_t page_size, max_pages, B, Hq, Hkv, D, dtype;
+  float sm_scale;
+} tread_paged_attn_args;
+int tread_paged_attn(const tread_paged_attn_args* args, tread_stream_t stream);
 
 /*
  * The next token's logits, adjusted (no counterpart in the reference, which is greedy on raw logits,
@@ -321,13 +333,19 @@ int tread_paged_attn(const void* q, int64_t q_ld, const void* k_pages, const voi
  *   allowed     : device int32 [B, ceil(V / 32)] at row stride allowed_ld (0: one mask for all rows),
  *                 bit v % 32 of word v / 32 set: v is allowed; NULL: every token is
  */
-int tread_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, int B, int V,
-                        const int64_t* tokens, int64_t tokens_ld, int max_tokens, const int64_t* lens,
-                        const int64_t* prompt_lens, const float* repetition, float repetition_all,
-                        const float* presence, float presence_all, const float* frequency,
-                        float frequency_all, const int64_t* bias_ids, int64_t bias_ids_ld,
-                        const float* bias, int64_t bias_ld, int num_bias, const int32_t* allowed,
-                        int64_t allowed_ld, int dtype, int out_dtype, tread_stream_t stream);
+typedef struct {
+  const void* logits;
+  void* out;
+  const int64_t *tokens, *lens, *prompt_lens;
+  const float *repetition, *presence, *frequency;
+  const int64_t* bias_ids;
+  const float* bias;
+  const int32_t* allowed;
+  int64_t ld, ld_out, tokens_ld, bias_ids_ld, bias_ld, allowed_ld;
+  int32_t B, V, max_tokens, num_bias, dtype, out_dtype;
+  float repetition_all, presence_all, frequency_all;
+} tread_adjust_logits_args;
+int tread_adjust_logits(const tread_adjust_logits_args* args, tread_stream_t stream);
 
 /*
  * Block-store tier transfers (pinned host <-> HBM), stream-ordered DMA copies.

@@ -7,12 +7,11 @@ from tread_b200 import _capi as C
 def _append_call(**over):
     a = dict(k=256, k_ld=1024, k_sh=128, v=256, v_ld=1024, v_sh=128, q=256, q_ld=1024, q_sh=128, q_out=256, kp=256,
              vp=256, ps=2 * 16 * 128, hs=16 * 128, N=8, page=16, table=256, t_ld=4, S=4, P=4, seq=None, pos=256,
-             rpos=None, R=3, Hq=4, Hkv=2, D=128, inv=256, scale=1.0, dtype=C.TREAD_BF16)
+             rpos=None, R=3, Hq=4, Hkv=2, D=128, inv=256, scale=1.0, err=None, dtype=C.TREAD_BF16)
     a.update(over)
-    return C.lib().tread_paged_append(
-        a["k"], a["k_ld"], a["k_sh"], a["v"], a["v_ld"], a["v_sh"], a["q"], a["q_ld"], a["q_sh"], a["q_out"], a["kp"],
-        a["vp"], a["ps"], a["hs"], a["N"], a["page"], a["table"], a["t_ld"], a["S"], a["P"], a["seq"], a["pos"],
-        a["rpos"], a["R"], a["Hq"], a["Hkv"], a["D"], a["inv"], a["scale"], a["dtype"], None, None)
+    return C.lib().tread_paged_append(C.PAGED_APPEND.pack(*(a[n] or 0 for n in (
+        "k v q q_out kp vp table seq pos rpos inv err k_ld k_sh v_ld v_sh q_ld q_sh ps hs N t_ld page S P R Hq Hkv D dtype "
+        "scale").split())), None)
 
 
 @pytest.mark.parametrize("over,needle", [
@@ -30,12 +29,12 @@ def test_paged_append_rejects_bad_arguments(over, needle):
 
 def _attn_call(**over):
     a = dict(q=256, q_ld=512, kp=256, vp=256, ps=2 * 16 * 128, hs=16 * 128, N=8, page=16, table=256, t_ld=4, P=4,
-             lens=256, B=3, Hq=4, Hkv=2, D=128, scale=0.1, out=256, dtype=C.TREAD_BF16, ws=256, ws_bytes=None)
+             lens=256, B=3, Hq=4, Hkv=2, D=128, scale=0.1, out=256, dtype=C.TREAD_BF16, ws=256, ws_bytes=None, err=None)
     a.update(over)
     n = C.lib().tread_paged_attn_workspace_bytes(4, 2, 128) if a["ws_bytes"] is None else a["ws_bytes"]
-    return C.lib().tread_paged_attn(
-        a["q"], a["q_ld"], a["kp"], a["vp"], a["ps"], a["hs"], a["N"], a["page"], a["table"], a["t_ld"], a["P"],
-        a["lens"], a["B"], a["Hq"], a["Hkv"], a["D"], a["scale"], a["out"], a["dtype"], None, a["ws"], n, None)
+    a["ws_bytes"] = n
+    return C.lib().tread_paged_attn(C.PAGED_ATTN.pack(*(a[k] or 0 for k in (
+        "q kp vp out table lens err ws q_ld ps hs N t_ld ws_bytes page P B Hq Hkv D dtype scale").split())), None)
 
 
 @pytest.mark.parametrize("over,needle", [
@@ -56,10 +55,9 @@ def _logits_call(**over):
              rep_all=1.2, pres=None, pres_all=0.0, freq=None, freq_all=0.0, ids=256, ids_ld=2, bias=256, bias_ld=2,
              nb=2, allowed=256, al_ld=4, dtype=C.TREAD_BF16, odt=C.TREAD_F32)
     a.update(over)
-    return C.lib().tread_adjust_logits(
-        a["x"], a["ld"], a["out"], a["ld_out"], a["B"], a["V"], a["tok"], a["tok_ld"], a["H"], a["lens"], a["plens"],
-        a["rep"], a["rep_all"], a["pres"], a["pres_all"], a["freq"], a["freq_all"], a["ids"], a["ids_ld"], a["bias"],
-        a["bias_ld"], a["nb"], a["allowed"], a["al_ld"], a["dtype"], a["odt"], None)
+    return C.lib().tread_adjust_logits(C.ADJUST_LOGITS.pack(*(a[k] or 0 for k in (
+        "x out tok lens plens rep pres freq ids bias allowed ld ld_out tok_ld ids_ld bias_ld al_ld B V H nb dtype odt "
+        "rep_all pres_all freq_all").split())), None)
 
 
 @pytest.mark.parametrize("over,needle", [
@@ -71,6 +69,36 @@ def _logits_call(**over):
 def test_adjust_logits_rejects_bad_arguments(over, needle):
     assert _logits_call(**over) == 1
     assert needle in C.lib().tread_last_error().decode()
+
+
+def test_null_arguments_are_refused():
+    for name in ("tread_paged_append", "tread_paged_attn", "tread_adjust_logits"):
+        assert getattr(C.lib(), name)(None, None) == 1
+        assert "null" in C.lib().tread_last_error().decode()
+
+
+def test_packed_structs_have_the_headers_layout(tmp_path):
+    """Sizes and last fields' offsets, as the C compiler lays the structs out."""
+    import os
+    import subprocess
+
+    from conftest import ROOT
+
+    src = tmp_path / "layout.c"
+    src.write_text("""#include <stddef.h>
+        #include <stdio.h>
+        #include "tread_b200.h"
+        int main(void) {
+          printf("%zu %zu %zu %zu %zu %zu\\n", sizeof(tread_paged_append_args),
+                 offsetof(tread_paged_append_args, attn_scaling), sizeof(tread_paged_attn_args),
+                 offsetof(tread_paged_attn_args, sm_scale), sizeof(tread_adjust_logits_args),
+                 offsetof(tread_adjust_logits_args, frequency_all));
+          return 0;
+        }""")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], capture_output=True, check=True).stdout.split()]
+    append, attn, logits = C.PAGED_APPEND.size, C.PAGED_ATTN.size, C.ADJUST_LOGITS.size
+    assert got == [append, append - 8, attn, attn - 4, logits, logits - 8]
 
 
 def test_empty_calls_are_noops():

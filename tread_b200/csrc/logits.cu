@@ -17,22 +17,7 @@ constexpr int kThreads = 256;
 constexpr int kSlice = 8192;
 constexpr unsigned kPrompt = 0x80000000u;  // set in a counter: the token is in the prompt
 
-struct LogitsArgs {
-  const void* logits;
-  void* out;
-  long long ld, ld_out, tokens_ld, allowed_ld, bias_ld, bias_ids_ld;
-  const int64_t* tokens;
-  const int64_t* lens;
-  const int64_t* prompt_lens;
-  const float* repetition;  // [B], or NULL: the value beside it
-  const float* presence;
-  const float* frequency;
-  float repetition_all, presence_all, frequency_all;
-  const int64_t* bias_ids;
-  const float* bias;
-  const int32_t* allowed;
-  int V, max_tokens, num_bias;
-};
+using LogitsArgs = tread_adjust_logits_args;
 
 __device__ __forceinline__ void store(void* out, long long i, int dtype, float x) {
   if (dtype == TREAD_F32)
@@ -114,34 +99,26 @@ int launch(const LogitsArgs& a, int B, int out_dtype, cudaStream_t st) {
 }  // namespace
 }  // namespace tread
 
-extern "C" int tread_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, int B, int V,
-                                   const int64_t* tokens, int64_t tokens_ld, int max_tokens, const int64_t* lens,
-                                   const int64_t* prompt_lens, const float* repetition, float repetition_all,
-                                   const float* presence, float presence_all, const float* frequency,
-                                   float frequency_all, const int64_t* bias_ids, int64_t bias_ids_ld,
-                                   const float* bias, int64_t bias_ld, int num_bias, const int32_t* allowed,
-                                   int64_t allowed_ld, int dtype, int out_dtype, tread_stream_t stream) {
+extern "C" int tread_adjust_logits(const tread_adjust_logits_args* args, tread_stream_t stream) {
   using namespace tread;
-  TREAD_CHECK_ARG(B >= 0 && V >= 0, "adjust_logits: B < 0 or V < 0");
-  if (B == 0 || V == 0) return TREAD_OK;
-  TREAD_CHECK_ARG(logits && out, "adjust_logits: null pointer");
-  TREAD_CHECK_ARG(B <= 65535, "adjust_logits: more than 65535 rows");
-  TREAD_CHECK_ARG(dtype_size(dtype) != 0 && dtype_size(out_dtype) != 0, "adjust_logits: unknown dtype %d or %d", dtype,
-                  out_dtype);
-  TREAD_CHECK_ARG(B == 1 || (ld >= V && ld_out >= V), "adjust_logits: row stride below the vocabulary");
-  TREAD_CHECK_ARG(max_tokens >= 0 && (!tokens || B == 1 || tokens_ld >= max_tokens), "adjust_logits: bad history");
-  TREAD_CHECK_ARG(num_bias >= 0 && (num_bias == 0 || (bias_ids && bias)), "adjust_logits: bad biases");
-  TREAD_CHECK_ARG(repetition || repetition_all > 0.f, "adjust_logits: repetition must be above 0");
-  LogitsArgs a;
-  a.logits = logits, a.out = out, a.ld = ld, a.ld_out = ld_out, a.tokens_ld = tokens_ld, a.allowed_ld = allowed_ld;
-  a.bias_ld = bias_ld, a.bias_ids_ld = bias_ids_ld, a.tokens = tokens, a.lens = lens, a.prompt_lens = prompt_lens;
-  a.repetition = repetition, a.presence = presence, a.frequency = frequency, a.repetition_all = repetition_all;
-  a.presence_all = presence_all, a.frequency_all = frequency_all, a.bias_ids = bias_ids, a.bias = bias;
-  a.allowed = allowed, a.V = V, a.max_tokens = tokens ? max_tokens : 0, a.num_bias = num_bias;
+  TREAD_CHECK_ARG(args, "adjust_logits: null arguments");
+  LogitsArgs a = *args;
+  TREAD_CHECK_ARG(a.B >= 0 && a.V >= 0, "adjust_logits: B < 0 or V < 0");
+  if (a.B == 0 || a.V == 0) return TREAD_OK;
+  TREAD_CHECK_ARG(a.logits && a.out, "adjust_logits: null pointer");
+  TREAD_CHECK_ARG(a.B <= 65535, "adjust_logits: more than 65535 rows");
+  TREAD_CHECK_ARG(dtype_size(a.dtype) != 0 && dtype_size(a.out_dtype) != 0, "adjust_logits: unknown dtype %d or %d",
+                  a.dtype, a.out_dtype);
+  TREAD_CHECK_ARG(a.B == 1 || (a.ld >= a.V && a.ld_out >= a.V), "adjust_logits: row stride below the vocabulary");
+  TREAD_CHECK_ARG(a.max_tokens >= 0 && (!a.tokens || a.B == 1 || a.tokens_ld >= a.max_tokens),
+                  "adjust_logits: bad history");
+  TREAD_CHECK_ARG(a.num_bias >= 0 && (a.num_bias == 0 || (a.bias_ids && a.bias)), "adjust_logits: bad biases");
+  TREAD_CHECK_ARG(a.repetition || a.repetition_all > 0.f, "adjust_logits: repetition must be above 0");
+  if (!a.tokens) a.max_tokens = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case TREAD_BF16: return launch<__nv_bfloat16>(a, B, out_dtype, st);
-    case TREAD_F16: return launch<__half>(a, B, out_dtype, st);
-    default: return launch<float>(a, B, out_dtype, st);
+  switch (a.dtype) {
+    case TREAD_BF16: return launch<__nv_bfloat16>(a, a.B, a.out_dtype, st);
+    case TREAD_F16: return launch<__half>(a, a.B, a.out_dtype, st);
+    default: return launch<float>(a, a.B, a.out_dtype, st);
   }
 }

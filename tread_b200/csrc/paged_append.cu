@@ -22,26 +22,7 @@ constexpr int kMaxHalf = 128;
 constexpr int kMaxTile = 16;  // rows per CTA
 constexpr int kUnroll = 4;    // pieces (one head of one row) in flight per thread
 
-struct AppendArgs {
-  const void* k;
-  const void* v;
-  const void* q;
-  long long k_ld, k_sh, v_ld, v_sh, q_ld, q_sh;
-  void* q_out;
-  void* k_pages;
-  void* v_pages;
-  long long page_stride, head_stride, num_pages;
-  const int32_t* table;
-  long long table_ld;
-  int num_seqs, max_pages, page_size;
-  const int32_t* seq;
-  const int64_t* pos;
-  const int64_t* rope_pos;
-  int R, Hq, Hkv, D;
-  const float* inv_freq;
-  float scale;
-  unsigned* err;
-};
+using AppendArgs = tread_paged_append_args;
 
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
@@ -70,7 +51,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
           ok = id >= 0 && id < a.num_pages;
           if (ok) dst = id * a.page_stride + (p - pg * a.page_size) * a.D;
         }
-        if (!ok && a.err) atomicOr(a.err, 1u);
+        if (!ok && a.err_flag) atomicOr(static_cast<unsigned*>(a.err_flag), 1u);
       }
     }
     s_dst[threadIdx.x] = dst;
@@ -83,7 +64,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
         const double half_turns = (double)a.rope_pos[r] * (double)a.inv_freq[i] * 0.31830988618379067154;
         float sn, cs;
         sincospif((float)(half_turns - 2.0 * rint(0.5 * half_turns)), &sn, &cs);
-        s_cs[w] = make_float2(cs * a.scale, sn * a.scale);
+        s_cs[w] = make_float2(cs * a.attn_scaling, sn * a.attn_scaling);
       }
     }
   }
@@ -172,42 +153,34 @@ int launch(const AppendArgs& a, bool vec, cudaStream_t st) {
 }  // namespace
 }  // namespace tread
 
-extern "C" int tread_paged_append(const void* k, int64_t k_ld, int64_t k_sh, const void* v, int64_t v_ld, int64_t v_sh,
-                                  const void* q, int64_t q_ld, int64_t q_sh, void* q_out, void* k_pages, void* v_pages,
-                                  int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
-                                  const int32_t* table, int64_t table_ld, int num_seqs, int max_pages,
-                                  const int32_t* seq, const int64_t* pos, const int64_t* rope_pos, int R, int Hq,
-                                  int Hkv, int D, const float* inv_freq, float attn_scaling, int dtype,
-                                  void* err_flag, tread_stream_t stream) {
+extern "C" int tread_paged_append(const tread_paged_append_args* args, tread_stream_t stream) {
   using namespace tread;
-  TREAD_CHECK_ARG(R >= 0, "paged_append: R < 0");
-  if (R == 0) return TREAD_OK;
-  TREAD_CHECK_ARG(k && v && k_pages && v_pages && pos, "paged_append: null pointer");
-  TREAD_CHECK_ARG(Hkv > 0 && Hkv <= 65535 && Hq >= 0 && Hq <= 65535, "paged_append: bad heads Hq=%d Hkv=%d", Hq, Hkv);
-  TREAD_CHECK_ARG(D >= 2 && D % 2 == 0 && D / 2 <= kMaxHalf, "paged_append: bad head_dim %d", D);
-  TREAD_CHECK_ARG(Hq == 0 || (q && q_out && inv_freq), "paged_append: query heads need q, q_out and inv_freq");
-  TREAD_CHECK_ARG(dtype_size(dtype) != 0, "paged_append: unknown dtype %d", dtype);
-  TREAD_CHECK_ARG(page_size > 0 && num_pages >= 0 && num_pages <= INT32_MAX &&
-                      (num_pages <= 1 || page_stride >= (int64_t)page_size * D) &&
-                      (Hkv == 1 || head_stride >= (int64_t)page_size * D),
+  TREAD_CHECK_ARG(args, "paged_append: null arguments");
+  AppendArgs a = *args;
+  TREAD_CHECK_ARG(a.R >= 0, "paged_append: R < 0");
+  if (a.R == 0) return TREAD_OK;
+  TREAD_CHECK_ARG(a.k && a.v && a.k_pages && a.v_pages && a.pos, "paged_append: null pointer");
+  TREAD_CHECK_ARG(a.Hkv > 0 && a.Hkv <= 65535 && a.Hq >= 0 && a.Hq <= 65535, "paged_append: bad heads Hq=%d Hkv=%d",
+                  a.Hq, a.Hkv);
+  TREAD_CHECK_ARG(a.D >= 2 && a.D % 2 == 0 && a.D / 2 <= kMaxHalf, "paged_append: bad head_dim %d", a.D);
+  TREAD_CHECK_ARG(a.Hq == 0 || (a.q && a.q_out && a.inv_freq), "paged_append: query heads need q, q_out and inv_freq");
+  TREAD_CHECK_ARG(dtype_size(a.dtype) != 0, "paged_append: unknown dtype %d", a.dtype);
+  TREAD_CHECK_ARG(a.page_size > 0 && a.num_pages >= 0 && a.num_pages <= INT32_MAX &&
+                      (a.num_pages <= 1 || a.page_stride >= (int64_t)a.page_size * a.D) &&
+                      (a.Hkv == 1 || a.head_stride >= (int64_t)a.page_size * a.D),
                   "paged_append: bad page geometry");
-  TREAD_CHECK_ARG(num_seqs >= 0 && max_pages >= 0 && (table || num_seqs == 0 || max_pages == 0) &&
-                      (num_seqs <= 1 || table_ld >= max_pages),
+  TREAD_CHECK_ARG(a.num_seqs >= 0 && a.max_pages >= 0 && (a.table || a.num_seqs == 0 || a.max_pages == 0) &&
+                      (a.num_seqs <= 1 || a.table_ld >= a.max_pages),
                   "paged_append: bad page table");
-  TREAD_CHECK_ARG(seq || R <= num_seqs, "paged_append: %d rows without seq, but %d sequences", R, num_seqs);
-  AppendArgs a;
-  a.k = k, a.v = v, a.q = q, a.k_ld = k_ld, a.k_sh = k_sh, a.v_ld = v_ld, a.v_sh = v_sh, a.q_ld = q_ld, a.q_sh = q_sh;
-  a.q_out = q_out, a.k_pages = k_pages, a.v_pages = v_pages, a.page_stride = page_stride, a.head_stride = head_stride;
-  a.num_pages = num_pages, a.table = table, a.table_ld = table_ld, a.num_seqs = num_seqs, a.max_pages = max_pages;
-  a.page_size = page_size, a.seq = seq, a.pos = pos, a.rope_pos = rope_pos ? rope_pos : pos, a.R = R, a.Hq = Hq;
-  a.Hkv = Hkv, a.D = D, a.inv_freq = inv_freq, a.scale = attn_scaling, a.err = static_cast<unsigned*>(err_flag);
+  TREAD_CHECK_ARG(a.seq || a.R <= a.num_seqs, "paged_append: %d rows without seq, but %d sequences", a.R, a.num_seqs);
+  if (!a.rope_pos) a.rope_pos = a.pos;
   // 16-byte vectors where every head of every row starts on a 16-byte boundary, else single elements
-  const int64_t ve = 16 / (int64_t)dtype_size(dtype);
-  const bool vec = (D / 2) % ve == 0 && (k_ld | k_sh | v_ld | v_sh | page_stride | head_stride) % ve == 0 &&
-                   (Hq == 0 || (q_ld | q_sh) % ve == 0) && aligned16(k) && aligned16(v) && aligned16(k_pages) &&
-                   aligned16(v_pages) && (Hq == 0 || (aligned16(q) && aligned16(q_out)));
+  const int64_t ve = 16 / (int64_t)dtype_size(a.dtype);
+  const bool vec = (a.D / 2) % ve == 0 && (a.k_ld | a.k_sh | a.v_ld | a.v_sh | a.page_stride | a.head_stride) % ve == 0 &&
+                   (a.Hq == 0 || (a.q_ld | a.q_sh) % ve == 0) && aligned16(a.k) && aligned16(a.v) &&
+                   aligned16(a.k_pages) && aligned16(a.v_pages) && (a.Hq == 0 || (aligned16(a.q) && aligned16(a.q_out)));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  switch (dtype) {
+  switch (a.dtype) {
     case TREAD_BF16: return launch<__nv_bfloat16>(a, vec, st);
     case TREAD_F16: return launch<__half>(a, vec, st);
     default: return launch<float>(a, vec, st);

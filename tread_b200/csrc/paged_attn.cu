@@ -34,15 +34,8 @@ constexpr int kMaxCtas = 384;  // shares at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // the running maximum may lag by 2^8: weights stay far inside fp16's range
 
-struct DecodeArgs {
-  const void* q;
-  const void* k_pages;
-  const void* v_pages;
-  void* out;
-  long long q_ld, page_stride, head_stride, num_pages, table_ld;
-  const int32_t* table;
-  const int64_t* lens;
-  int B, Hq, Hkv, G, max_pages, page_size;
+struct DecodeArgs : tread_paged_attn_args {
+  int G;
   float scale_log2;
   unsigned* err;
   int4* desc;   // [kMaxCtas] {parts of the item that starts in this CTA and ends in another, b, g, slot}
@@ -683,52 +676,49 @@ extern "C" size_t tread_paged_attn_workspace_bytes(int Hq, int Hkv, int D) {
   return align256(kMaxCtas * sizeof(int4)) + align256(states * sizeof(float2)) + states * D * sizeof(float);
 }
 
-extern "C" int tread_paged_attn(const void* q, int64_t q_ld, const void* k_pages, const void* v_pages,
-                                int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
-                                const int32_t* table, int64_t table_ld, int max_pages, const int64_t* lens, int B,
-                                int Hq, int Hkv, int D, float sm_scale, void* out, int dtype, void* err_flag,
-                                void* workspace, size_t workspace_bytes, tread_stream_t stream) {
+extern "C" int tread_paged_attn(const tread_paged_attn_args* args, tread_stream_t stream) {
   using namespace tread;
-  TREAD_CHECK_ARG(B >= 0, "paged_attn: B < 0");
-  if (B == 0) return TREAD_OK;
-  TREAD_CHECK_ARG(q && k_pages && v_pages && lens && out, "paged_attn: null pointer");
-  TREAD_CHECK_ARG(Hq > 0 && Hkv > 0 && Hkv <= 65535 && Hq % Hkv == 0 && Hq / Hkv <= 16,
-                  "paged_attn: bad heads Hq=%d Hkv=%d", Hq, Hkv);
-  TREAD_CHECK_ARG(D == 64 || D == 128 || D == 256, "paged_attn: head_dim %d not in {64,128,256}", D);
-  const int64_t es = (int64_t)dtype_size(dtype);
-  TREAD_CHECK_ARG(es != 0, "paged_attn: unknown dtype %d", dtype);
-  TREAD_CHECK_ARG(page_size > 0 && num_pages >= 0 && num_pages <= INT32_MAX &&
-                      (num_pages <= 1 || page_stride >= (int64_t)page_size * D) &&
-                      (Hkv == 1 || head_stride >= (int64_t)page_size * D),
+  TREAD_CHECK_ARG(args, "paged_attn: null arguments");
+  DecodeArgs a;
+  static_cast<tread_paged_attn_args&>(a) = *args;
+  TREAD_CHECK_ARG(a.B >= 0, "paged_attn: B < 0");
+  if (a.B == 0) return TREAD_OK;
+  TREAD_CHECK_ARG(a.q && a.k_pages && a.v_pages && a.lens && a.out, "paged_attn: null pointer");
+  TREAD_CHECK_ARG(a.Hq > 0 && a.Hkv > 0 && a.Hkv <= 65535 && a.Hq % a.Hkv == 0 && a.Hq / a.Hkv <= 16,
+                  "paged_attn: bad heads Hq=%d Hkv=%d", a.Hq, a.Hkv);
+  TREAD_CHECK_ARG(a.D == 64 || a.D == 128 || a.D == 256, "paged_attn: head_dim %d not in {64,128,256}", a.D);
+  const int64_t es = (int64_t)dtype_size(a.dtype);
+  TREAD_CHECK_ARG(es != 0, "paged_attn: unknown dtype %d", a.dtype);
+  TREAD_CHECK_ARG(a.page_size > 0 && a.num_pages >= 0 && a.num_pages <= INT32_MAX &&
+                      (a.num_pages <= 1 || a.page_stride >= (int64_t)a.page_size * a.D) &&
+                      (a.Hkv == 1 || a.head_stride >= (int64_t)a.page_size * a.D),
                   "paged_attn: bad page geometry");
-  TREAD_CHECK_ARG(max_pages >= 0 && (table || max_pages == 0) && (B <= 1 || table_ld >= max_pages),
+  TREAD_CHECK_ARG(a.max_pages >= 0 && (a.table || a.max_pages == 0) && (a.B <= 1 || a.table_ld >= a.max_pages),
                   "paged_attn: bad page table");
-  TREAD_CHECK_ARG((int64_t)max_pages * page_size <= INT32_MAX - kUnit, "paged_attn: a sequence of 2^31 tokens or more");
-  TREAD_CHECK_ARG(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) &&
-                      ((q_ld | page_stride | head_stride) * es) % 16 == 0,
+  TREAD_CHECK_ARG((int64_t)a.max_pages * a.page_size <= INT32_MAX - kUnit,
+                  "paged_attn: a sequence of 2^31 tokens or more");
+  TREAD_CHECK_ARG(aligned16(a.q) && aligned16(a.k_pages) && aligned16(a.v_pages) && aligned16(a.out) &&
+                      ((a.q_ld | a.page_stride | a.head_stride) * es) % 16 == 0,
                   "paged_attn: q, out and pages must lie on 16-byte boundaries");
-  TREAD_CHECK_ARG(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
-                      workspace_bytes >= tread_paged_attn_workspace_bytes(Hq, Hkv, D),
+  TREAD_CHECK_ARG(a.workspace && (reinterpret_cast<uintptr_t>(a.workspace) & 255u) == 0 &&
+                      a.workspace_bytes >= (int64_t)tread_paged_attn_workspace_bytes(a.Hq, a.Hkv, a.D),
                   "paged_attn: workspace too small or not 256-byte aligned");
   int device = 0, sms = 0;
   TREAD_CHECK_CUDA(cudaGetDevice(&device));
   TREAD_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-  DecodeArgs a;
-  a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_ld = q_ld, a.page_stride = page_stride;
-  a.head_stride = head_stride, a.num_pages = num_pages, a.table_ld = table_ld, a.table = table, a.lens = lens;
-  a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.max_pages = max_pages, a.page_size = page_size;
-  a.scale_log2 = sm_scale * kLog2e;
-  a.err = static_cast<unsigned*>(err_flag);
-  char* ws = static_cast<char*>(workspace);
+  a.G = a.Hq / a.Hkv;
+  a.scale_log2 = a.sm_scale * kLog2e;
+  a.err = static_cast<unsigned*>(a.err_flag);
+  char* ws = static_cast<char*>(a.workspace);
   a.desc = reinterpret_cast<int4*>(ws);
   ws += align256(kMaxCtas * sizeof(int4));
   a.ml = reinterpret_cast<float2*>(ws);
   ws += align256((size_t)kMaxCtas * 2 * a.G * sizeof(float2));
   a.part = reinterpret_cast<float*>(ws);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case TREAD_BF16: return dispatch<__nv_bfloat16>(D, a, sms, st);
-    case TREAD_F16: return dispatch<__half>(D, a, sms, st);
-    default: return dispatch<float>(D, a, sms, st);
+  switch (a.dtype) {
+    case TREAD_BF16: return dispatch<__nv_bfloat16>(a.D, a, sms, st);
+    case TREAD_F16: return dispatch<__half>(a.D, a, sms, st);
+    default: return dispatch<float>(a.D, a, sms, st);
   }
 }

@@ -497,26 +497,23 @@ def _index(t, n, dtype, name):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of length {n}")
 
 
-def _launch(fn, name, device, stream, *args):
-    """Call the library's fn(*args, stream) with `device` current."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, _stream_arg(stream, device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _stream_arg(stream, device))
-    C.check(rc, name)
+def _elsewhere(device, stream):
+    """The context in which a call on tensors of `device` has to run, or None where it is the current
+    one: launches and allocations go to the current device and stream."""
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the call's tensors on {device}")
+        return torch.cuda.stream(stream)
+    return None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
-def _empty(shape, dtype, device, stream):
-    """An uninitialised tensor that belongs to the stream that the launch goes to."""
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+def _launch(fn, name, device, args):
+    """Call the library's fn(args struct, current stream)."""
+    C.check(fn(args, torch._C._cuda_getCurrentRawStream(device.index)), name)
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, rope_pos=None, attn_scaling=1.0, q=None,
@@ -536,6 +533,11 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
       a zero query and sets bit 0.
     Returns the rotated queries [R, Hq, D] (q_out, which may be q itself), or None without q."""
     sp, sh = _pages(k_pages, v_pages)
+    device = k_pages.device
+    other = _elsewhere(device, stream)
+    if other is not None:
+        with other:
+            return paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out, err)
     N, Hkv, page_size, D = k_pages.shape
     C.same_device(k_pages, k=k, v=v, v_pages=v_pages, table=table, pos=pos, seq=seq, inv_freq=inv_freq,
                   rope_pos=rope_pos, q=q, q_out=q_out, err=err)
@@ -544,12 +546,12 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
     R = k.shape[0]
     if not (k.dtype == v.dtype == k_pages.dtype):
         raise TypeError("k, v and the pages must share a dtype")
-    ld = _table(table)
+    ld, (S, width) = _table(table), table.shape
     _index(pos, R, torch.int64, "pos")
     if seq is not None:
         _index(seq, R, torch.int32, "seq")
-    elif R > table.shape[0]:
-        raise ValueError(f"{R} rows without seq, but a table of {table.shape[0]} sequences")
+    elif R > S:
+        raise ValueError(f"{R} rows without seq, but a table of {S} sequences")
     if rope_pos is not None:
         _index(rope_pos, R, torch.int64, "rope_pos")
     if inv_freq is not None:
@@ -565,14 +567,15 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
             raise ValueError("q without inv_freq: nothing rotates it")
         Hq, q_ld, q_sh = q.shape[1], q.stride(0), q.stride(1)
         if q_out is None:
-            q_out = _empty(q.shape, q.dtype, q.device, stream)
+            q_out = torch.empty((R, Hq, D), dtype=q.dtype, device=device)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
             raise ValueError(f"q_out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
-    _launch(C.lib().tread_paged_append, "tread_paged_append", k_pages.device, stream, k.data_ptr(), k.stride(0),
-            k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _ptr(q), q_ld, q_sh, _ptr(q_out), k_pages.data_ptr(),
-            v_pages.data_ptr(), sp, sh, N, page_size, table.data_ptr(), ld, table.shape[0], table.shape[1], _ptr(seq),
-            pos.data_ptr(), _ptr(rope_pos), R, Hq, Hkv, D, _ptr(inv_freq), float(attn_scaling),
-            C.dtype_code(k.dtype), _ptr(err))
+    k_ld, k_sh, _ = k.stride()
+    v_ld, v_sh, _ = v.stride()
+    _launch(C.lib().tread_paged_append, "tread_paged_append", device, C.PAGED_APPEND.pack(
+        k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
+        _ptr(seq), pos.data_ptr(), _ptr(rope_pos), _ptr(inv_freq), _ptr(err), k_ld, k_sh, v_ld, v_sh, q_ld, q_sh, sp, sh,
+        N, ld, page_size, S, width, R, Hq, Hkv, D, C.dtype_code(k.dtype), attn_scaling))
     return q_out
 
 
@@ -584,26 +587,33 @@ def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=No
     err: device error word; a length that the table has no pages for gives a row of zeros and sets bit
     1, and so does a page id outside the pool, whose keys count as masked. Returns out [B, Hq, D]."""
     sp, sh = _pages(k_pages, v_pages)
+    device = k_pages.device
+    other = _elsewhere(device, stream)
+    if other is not None:
+        with other:
+            return paged_attn(q, k_pages, v_pages, table, lens, out, sm_scale, err)
     N, Hkv, page_size, D = k_pages.shape
     C.same_device(k_pages, q=q, v_pages=v_pages, table=table, lens=lens, out=out, err=err)
     if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != D) or (
             q.dtype != k_pages.dtype):
         raise ValueError(f"q must be [B, Hq, {D}] of the pages' dtype with contiguous rows")
-    B, Hq = q.shape[0], q.shape[1]
-    ld = _table(table)
-    if table.shape[0] != B:
+    B, Hq, _ = q.shape
+    ld, (rows, width) = _table(table), table.shape
+    if rows != B:
         raise ValueError(f"table must have a row for each of the {B} sequences")
     _index(lens, B, torch.int64, "lens")
     if out is None:
-        out = _empty(q.shape, q.dtype, q.device, stream)
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
     lib = C.lib()
-    ws = _empty((lib.tread_paged_attn_workspace_bytes(Hq, Hkv, D),), torch.uint8, q.device, stream)
-    _launch(lib.tread_paged_attn, "tread_paged_attn", q.device, stream, q.data_ptr(), q.stride(0), k_pages.data_ptr(),
-            v_pages.data_ptr(), sp, sh, N, page_size, table.data_ptr(), ld, table.shape[1], lens.data_ptr(), B, Hq, Hkv,
-            D, D ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), C.dtype_code(q.dtype), _ptr(err),
-            ws.data_ptr(), ws.numel())
+    # one workspace a call, from the allocator: calls of several streams, threads and graphs share none
+    nbytes = lib.tread_paged_attn_workspace_bytes(Hq, Hkv, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _launch(lib.tread_paged_attn, "tread_paged_attn", device, C.PAGED_ATTN.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), _ptr(err),
+        ws.data_ptr(), q.stride(0), sp, sh, N, ld, nbytes, page_size, width, B, Hq, Hkv, D, C.dtype_code(q.dtype),
+        D ** -0.5 if sm_scale is None else sm_scale))
     return out
 
 
@@ -613,8 +623,8 @@ def _per_row(x, B, name, device):
         if x.device != device:
             raise ValueError(f"{name} is on {x.device}, the logits on {device}")
         _index(x, B, torch.float32, name)
-        return x.data_ptr(), 0.0
-    return None, float(x)
+        return x.data_ptr(), 1.0
+    return 0, float(x)
 
 
 def _by_row(t, B, width, dtype, name):
@@ -643,8 +653,13 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
     C.require_cuda(logits, "logits")
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [B, V] with unit column stride")
-    B, V = logits.shape
     device = logits.device
+    other = _elsewhere(device, stream)
+    if other is not None:
+        with other:
+            return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
+                                 allowed, out)
+    B, V = logits.shape
     C.same_device(logits, tokens=tokens, lens=lens, prompt_lens=prompt_lens, bias_ids=bias_ids, bias=bias,
                   allowed=allowed, out=out)
     H = tok_ld = 0
@@ -660,7 +675,7 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
             _index(t, B, torch.int64, name)
     rep, pres, freq = (_per_row(x, B, n, device) for x, n in ((repetition, "repetition"), (presence, "presence"),
                                                               (frequency, "frequency")))
-    if rep[0] is None and not rep[1] > 0:
+    if not rep[1] > 0:
         raise ValueError(f"repetition must be above 0, got {repetition}")
     nb = ids_ld = bias_ld = 0
     if (bias is None) != (bias_ids is None):
@@ -670,15 +685,15 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
         ids_ld, bias_ld = _by_row(bias_ids, B, nb, torch.int64, "bias_ids"), _by_row(bias, B, nb, torch.float32, "bias")
     allowed_ld = 0 if allowed is None else _by_row(allowed, B, (V + 31) // 32, torch.int32, "allowed")
     if out is None:
-        out = _empty((B, V), torch.float32, device, stream)
+        out = torch.empty((B, V), dtype=torch.float32, device=device)
     elif out.shape != (B, V) or (V > 1 and out.stride(1) != 1):
         raise ValueError(f"out must be [{B}, {V}] with unit column stride")
     elif out.data_ptr() == logits.data_ptr() and (out.dtype != logits.dtype or out.stride(0) != logits.stride(0)):
         raise ValueError("out over logits must have their dtype and row stride")
-    _launch(C.lib().tread_adjust_logits, "tread_adjust_logits", device, stream, logits.data_ptr(), logits.stride(0),
-            out.data_ptr(), out.stride(0), B, V, _ptr(tokens), tok_ld, H, _ptr(lens), _ptr(prompt_lens),
-            rep[0], rep[1] if rep[0] is None else 1.0, pres[0], pres[1], freq[0], freq[1], _ptr(bias_ids), ids_ld,
-            _ptr(bias), bias_ld, nb, _ptr(allowed), allowed_ld, C.dtype_code(logits.dtype), C.dtype_code(out.dtype))
+    _launch(C.lib().tread_adjust_logits, "tread_adjust_logits", device, C.ADJUST_LOGITS.pack(
+        logits.data_ptr(), out.data_ptr(), _ptr(tokens), _ptr(lens), _ptr(prompt_lens), rep[0], pres[0], freq[0],
+        _ptr(bias_ids), _ptr(bias), _ptr(allowed), logits.stride(0), out.stride(0), tok_ld, ids_ld, bias_ld, allowed_ld, B,
+        V, H, nb, C.dtype_code(logits.dtype), C.dtype_code(out.dtype), rep[1], pres[1], freq[1]))
     return out
 
 
