@@ -153,6 +153,16 @@ def test_long_histories():
     _check(kernels.adjust_logits(logits, **kw), logits, **kw)
 
 
+def test_many_biases_and_every_row_offset():
+    """More biases than threads, rows that start at every offset from a 16-byte boundary, vectors of the
+    mask that straddle its words, vocabularies of one vector and less."""
+    for V in (1003, 2051, 40, 9, 3):
+        logits, kw = _case(9, V, 64, BF, V, biases=700)
+        _check(kernels.adjust_logits(logits, **kw), logits, **kw)
+        f, kf = _case(5, V, 64, FP, V + 1, biases=300)
+        _check(kernels.adjust_logits(f, out=torch.empty(5, V, dtype=HF, device=DEV), **kf), f, **kf)
+
+
 def test_graph_replay_and_streams():
     logits, kw = _case(4, 20000, 100, BF, 14)
     want = kernels.adjust_logits(logits, **kw)

@@ -6,18 +6,43 @@
 //   x -= frequency * n[v] + presence * (n[v] > 0);   x += bias of v;   v not allowed: x = -inf
 // in fp32, rounded once to the output's type. Ids outside [0, vocab) count for nothing (padding).
 //
-// A CTA owns a slice of a row's vocabulary. It counts the row's history into the slice's counters in shared
-// memory (whole numbers: the order of the atomics does not matter), then passes over the slice once.
+// Bound by reading the logits and writing the result. A CTA owns a slice of a row's vocabulary: it issues
+// the loads of all its logits, counts the row's whole history into counters of its slice in shared memory
+// while they fly (whole numbers: the order of the atomics does not matter), then finishes every logit in
+// one pass. Reading the history again for every slice costs L2 reads only, and no counters in memory that a
+// caller would have to keep or clear. Biased tokens are few: each is marked in its counter, left out of the
+// pass, and finished by the thread that marked it first, which adds its biases up in the list's order.
 #include "common.cuh"
 
 namespace tread {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSlice = 8192;
-constexpr unsigned kPrompt = 0x80000000u;  // set in a counter: the token is in the prompt
+constexpr int kVec = 8;          // consecutive logits of a thread
+constexpr int kMaxBias = 8192;   // 32 bits of ownership a thread
 
 using LogitsArgs = tread_adjust_logits_args;
+
+// A token's counter in 16 or 32 bits: how often the output holds it, and two marks.
+template <typename W>
+struct Counter {
+  static constexpr int kBits = sizeof(W) * 8;
+  static constexpr unsigned kPrompt = 1u << (kBits - 1);  // the prompt holds it
+  static constexpr unsigned kBiased = 1u << (kBits - 2);
+  static constexpr unsigned kCount = kBiased - 1;
+  // marks or counts token i of the slice; returns its counter as it was
+  static __device__ __forceinline__ unsigned mark(W* c, int i, unsigned what) {
+    if constexpr (sizeof(W) == 4) return atomicOr(reinterpret_cast<unsigned*>(c) + i, what);
+    const int shift = (i & 1) * 16;
+    return atomicOr(reinterpret_cast<unsigned*>(c) + (i >> 1), what << shift) >> shift;
+  }
+  static __device__ __forceinline__ void add(W* c, int i) {
+    if constexpr (sizeof(W) == 4)
+      atomicAdd(reinterpret_cast<unsigned*>(c) + i, 1u);
+    else
+      atomicAdd(reinterpret_cast<unsigned*>(c) + (i >> 1), 1u << ((i & 1) * 16));
+  }
+};
 
 __device__ __forceinline__ void store(void* out, long long i, int dtype, float x) {
   if (dtype == TREAD_F32)
@@ -29,71 +54,178 @@ __device__ __forceinline__ void store(void* out, long long i, int dtype, float x
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) adjust_logits_kernel(const __grid_constant__ LogitsArgs a, int out_dtype) {
-  extern __shared__ unsigned s_mem[];
-  unsigned* count = s_mem;                                  // [kSlice]
-  float* bias = reinterpret_cast<float*>(s_mem + kSlice);   // [kSlice], where biases are given
-  const int b = blockIdx.y, v0 = blockIdx.x * kSlice;
-  const int nv = a.V - v0 < kSlice ? a.V - v0 : kSlice;
-  for (int i = threadIdx.x; i < nv; i += kThreads) count[i] = 0;
-  if (a.num_bias)
-    for (int i = threadIdx.x; i < nv; i += kThreads) bias[i] = 0.f;
+__device__ __forceinline__ void store8(void* out, long long i, const float (&x)[kVec]) {
+  T* to = static_cast<T*>(out) + i;
+  constexpr int E = 16 / sizeof(T);
+#pragma unroll
+  for (int k = 0; k < kVec; k += E) {
+    Vec16<T> v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v.e[e] = Num<T>::from_f(x[k + e]);
+    st_stream(to + k, v.raw);
+  }
+}
+
+// VECS: vectors of kVec logits that a thread holds; a slice has VECS * kThreads of them at most
+template <typename T, typename W, int VECS>
+__global__ void __launch_bounds__(kThreads)
+    adjust_logits_kernel(const __grid_constant__ LogitsArgs a, int slice) {
+  using C = Counter<W>;
+  extern __shared__ __align__(16) unsigned char s_mem[];
+  W* count = reinterpret_cast<W*>(s_mem);  // of tokens first - kVec .. first + slice - 1
+  const int b = blockIdx.y;
+  const T* row = static_cast<const T*>(a.logits) + b * a.ld;
+  const long long out_row = b * a.ld_out;
+  // vectors start where the row's address is a multiple of 16 bytes: the first slice has the tokens before
+  const int head = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+  const int first = head + blockIdx.x * slice;               // token of the slice's first vector
+  const int begin = blockIdx.x == 0 ? 0 : first;
+  const int end = min(a.V, first + slice);
+  if (begin >= end) return;
+  const int vecs = end > first ? (end - first) / kVec : 0;  // whole ones; the rest of the row token by token
+  constexpr int L = kVec * sizeof(T) / 16;                   // 16-byte loads of a vector
+  int4 x[VECS][L];
+#pragma unroll
+  for (int k = 0; k < VECS; ++k) {
+    const int i = k * kThreads + threadIdx.x;
+    if (i < vecs) {
+#pragma unroll
+      for (int j = 0; j < L; ++j) x[k][j] = ld_stream(row + first + i * kVec + j * (16 / sizeof(T)));
+    }
+  }
+  const int origin = first - kVec;
+  for (int i = threadIdx.x; i < (int)((slice + kVec) * sizeof(W) / 16); i += kThreads)
+    reinterpret_cast<int4*>(s_mem)[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
   if (a.tokens) {
     long long len = a.lens ? a.lens[b] : a.max_tokens;
     len = len < 0 ? 0 : len > a.max_tokens ? a.max_tokens : len;
     const long long prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
-    for (long long i = threadIdx.x; i < len; i += kThreads) {
-      const long long v = a.tokens[b * a.tokens_ld + i] - v0;
-      if (v >= 0 && v < nv) {
-        if (i < prompt)
-          atomicOr(count + v, kPrompt);
+    const long long* ids = reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_ld;
+    constexpr int kAhead = 8;
+    for (int i0 = threadIdx.x; i0 < (int)len; i0 += kThreads * kAhead) {
+      long long v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) v[k] = i0 + k * kThreads < (int)len ? __ldg(ids + i0 + k * kThreads) : -1;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (v[k] < begin || v[k] >= end) continue;
+        if (i0 + k * kThreads < prompt)
+          C::mark(count, (int)v[k] - origin, C::kPrompt);
         else
-          atomicAdd(count + v, 1u);
+          C::add(count, (int)v[k] - origin);
       }
     }
   }
-  if (a.num_bias) {
-    // the same token twice: its first entry adds up all of them, in their order
-    const int64_t* ids = a.bias_ids + b * a.bias_ids_ld;
-    for (int i = threadIdx.x; i < a.num_bias; i += kThreads) {
-      const long long v = ids[i] - v0;
-      if (v < 0 || v >= nv) continue;
-      bool first = true;
-      for (int j = 0; j < i; ++j) first &= ids[j] != ids[i];
-      if (!first) continue;
-      float sum = 0.f;
-      for (int j = i; j < a.num_bias; ++j)
-        if (ids[j] == ids[i]) sum += a.bias[b * a.bias_ld + j];
-      bias[v] = sum;
-    }
+  unsigned mine = 0;  // biases whose token this thread marked first
+  const int64_t* bias_ids = a.bias_ids + b * a.bias_ids_ld;
+  for (int i = threadIdx.x, k = 0; i < a.num_bias; i += kThreads, ++k) {
+    const long long v = bias_ids[i];
+    if (v >= begin && v < end && !(C::mark(count, (int)v - origin, C::kBiased) & C::kBiased)) mine |= 1u << k;
   }
   __syncthreads();
   const float rep = a.repetition ? a.repetition[b] : a.repetition_all;
   const float pres = a.presence ? a.presence[b] : a.presence_all;
   const float freq = a.frequency ? a.frequency[b] : a.frequency_all;
-  for (int i = threadIdx.x; i < nv; i += kThreads) {
-    float x = Num<T>::to_f(static_cast<const T*>(a.logits)[b * a.ld + v0 + i]);
-    const unsigned c = count[i];
-    if (c) {
-      x = x > 0.f ? x / rep : x * rep;
-      const unsigned n = c & ~kPrompt;
-      if (n) x -= freq * (float)n + pres;
+  const unsigned* allowed = a.allowed ? reinterpret_cast<const unsigned*>(a.allowed) + b * a.allowed_ld : nullptr;
+  auto penalised = [&](float f, unsigned c) {
+    if (c & ~C::kBiased) {
+      f = f > 0.f ? f / rep : f * rep;
+      if (c & C::kCount) f -= freq * (float)(c & C::kCount) + pres;
     }
-    if (a.num_bias) x += bias[i];
-    if (a.allowed && !((a.allowed[b * a.allowed_ld + ((v0 + i) >> 5)] >> ((v0 + i) & 31)) & 1)) x = -INFINITY;
-    store(a.out, b * a.ld_out + v0 + i, out_dtype, x);
+    return f;
+  };
+  auto single = [&](int v) {  // one token, if it has no bias
+    const unsigned c = count[v - origin];
+    if (c & C::kBiased) return;
+    float f = penalised(Num<T>::to_f(row[v]), c);
+    if (allowed && !((allowed[v >> 5] >> (v & 31)) & 1)) f = -INFINITY;
+    store(a.out, out_row + v, a.out_dtype, f);
+  };
+  for (int k = 0; k < 32 && (mine >> k); ++k) {
+    if (!((mine >> k) & 1)) continue;
+    const long long v = bias_ids[k * kThreads + threadIdx.x];
+    float sum = 0.f;
+    for (int j = 0; j < a.num_bias; ++j)
+      if (bias_ids[j] == v) sum += a.bias[b * a.bias_ld + j];
+    float f = penalised(Num<T>::to_f(row[v]), count[v - origin]) + sum;
+    if (allowed && !((allowed[v >> 5] >> (v & 31)) & 1)) f = -INFINITY;
+    store(a.out, out_row + v, a.out_dtype, f);
+  }
+  if (threadIdx.x < first - begin && threadIdx.x < end) single(threadIdx.x);  // the first slice's tokens before
+  if (threadIdx.x < end - first - vecs * kVec) single(first + vecs * kVec + threadIdx.x);
+  const bool aligned =
+      (reinterpret_cast<uintptr_t>(a.out) + (out_row + first) * (a.out_dtype == TREAD_F32 ? 4 : 2)) % 16 == 0;
+#pragma unroll
+  for (int k = 0; k < VECS; ++k) {
+    const int i = k * kThreads + threadIdx.x;
+    if (i >= vecs) continue;
+    const int v = first + i * kVec;
+    float f[kVec];
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      Vec16<T> u;
+      u.raw = x[k][e * sizeof(T) / 16];
+      f[e] = Num<T>::to_f(u.e[e % (16 / sizeof(T))]);
+    }
+    unsigned biased = 0;
+    const int4* c = reinterpret_cast<const int4*>(count + (i + 1) * kVec);
+    unsigned w[sizeof(W) * 2];
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(W) / 2; ++j) *reinterpret_cast<int4*>(w + 4 * j) = c[j];
+    unsigned any = 0;
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(W) * 2; ++j) any |= w[j];
+    if (any) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const unsigned n = sizeof(W) == 4 ? w[e % (sizeof(W) * 2)] : (w[e / 2] >> ((e & 1) * 16)) & 0xffffu;
+        f[e] = penalised(f[e], n);
+        if (n & C::kBiased) biased |= 1u << e;
+      }
+    }
+    if (allowed) {
+      const int shift = v & 31;
+      unsigned bits = allowed[v >> 5] >> shift;
+      if (shift > 32 - kVec) bits |= allowed[(v >> 5) + 1] << (32 - shift);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (!((bits >> e) & 1)) f[e] = -INFINITY;
+    }
+    if (biased || !aligned) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (!((biased >> e) & 1)) store(a.out, out_row + v + e, a.out_dtype, f[e]);
+    } else if (a.out_dtype == TREAD_F32) {
+      store8<float>(a.out, out_row + v, f);
+    } else if (a.out_dtype == TREAD_BF16) {
+      store8<__nv_bfloat16>(a.out, out_row + v, f);
+    } else {
+      store8<__half>(a.out, out_row + v, f);
+    }
   }
 }
 
-template <typename T>
-int launch(const LogitsArgs& a, int B, int out_dtype, cudaStream_t st) {
-  const int smem = kSlice * (a.num_bias ? 8 : 4);
-  auto kern = adjust_logits_kernel<T>;
-  TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlice * 8));
-  kern<<<dim3((a.V + kSlice - 1) / kSlice, B), kThreads, smem, st>>>(a, out_dtype);
+template <typename T, typename W, int VECS>
+int launch(const LogitsArgs& a, cudaStream_t st) {
+  // slices of whole passes of the CTA, as small as leaves about four CTAs per SM
+  const int pass = kThreads * kVec;
+  const long long want = 592 / a.B > 1 ? 592 / a.B : 1;
+  int slice = (int)((a.V + want * pass - 1) / (want * pass)) * pass;
+  if (slice > VECS * pass) slice = VECS * pass;
+  const int smem = (slice + kVec) * (int)sizeof(W);
+  const int slices = (int)(((long long)a.V + slice - 1) / slice);  // the first one has up to kVec - 1 tokens more
+  auto kern = adjust_logits_kernel<T, W, VECS>;
+  if (smem > 48 * 1024) TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kern<<<dim3(slices, a.B), kThreads, smem, st>>>(a, slice);
   TREAD_CHECK_LAUNCH("adjust_logits_kernel");
   return TREAD_OK;
+}
+
+template <typename T, int VECS>
+int dispatch(const LogitsArgs& a, cudaStream_t st) {
+  // counters of 16 bits (14 of them the count) halve the shared memory; a longer history needs 32
+  return a.max_tokens < (1 << 14) ? launch<T, uint16_t, VECS>(a, st) : launch<T, uint32_t, VECS>(a, st);
 }
 
 }  // namespace
@@ -106,19 +238,20 @@ extern "C" int tread_adjust_logits(const tread_adjust_logits_args* args, tread_s
   TREAD_CHECK_ARG(a.B >= 0 && a.V >= 0, "adjust_logits: B < 0 or V < 0");
   if (a.B == 0 || a.V == 0) return TREAD_OK;
   TREAD_CHECK_ARG(a.logits && a.out, "adjust_logits: null pointer");
-  TREAD_CHECK_ARG(a.B <= 65535, "adjust_logits: more than 65535 rows");
+  TREAD_CHECK_ARG(a.B <= 65535 && a.V <= INT32_MAX - (1 << 20), "adjust_logits: more than 65535 rows or 2^31 - 2^20 tokens");
   TREAD_CHECK_ARG(dtype_size(a.dtype) != 0 && dtype_size(a.out_dtype) != 0, "adjust_logits: unknown dtype %d or %d",
                   a.dtype, a.out_dtype);
   TREAD_CHECK_ARG(a.B == 1 || (a.ld >= a.V && a.ld_out >= a.V), "adjust_logits: row stride below the vocabulary");
   TREAD_CHECK_ARG(a.max_tokens >= 0 && (!a.tokens || a.B == 1 || a.tokens_ld >= a.max_tokens),
                   "adjust_logits: bad history");
+  TREAD_CHECK_ARG(a.num_bias <= kMaxBias, "adjust_logits: more than %d biases", kMaxBias);
   TREAD_CHECK_ARG(a.num_bias >= 0 && (a.num_bias == 0 || (a.bias_ids && a.bias)), "adjust_logits: bad biases");
   TREAD_CHECK_ARG(a.repetition || a.repetition_all > 0.f, "adjust_logits: repetition must be above 0");
   if (!a.tokens) a.max_tokens = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (a.dtype) {
-    case TREAD_BF16: return launch<__nv_bfloat16>(a, a.B, a.out_dtype, st);
-    case TREAD_F16: return launch<__half>(a, a.B, a.out_dtype, st);
-    default: return launch<float>(a, a.B, a.out_dtype, st);
+    case TREAD_BF16: return dispatch<__nv_bfloat16, 8>(a, st);
+    case TREAD_F16: return dispatch<__half, 8>(a, st);
+    default: return dispatch<float, 4>(a, st);
   }
 }
