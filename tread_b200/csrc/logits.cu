@@ -8,16 +8,18 @@
 //
 // Bound by reading the logits and writing the result. A CTA owns a slice of a row's vocabulary: it issues
 // the loads of all its logits, counts the row's whole history into counters of its slice in shared memory
-// while they fly (whole numbers: the order of the atomics does not matter), then finishes every logit in
-// one pass. Reading the history again for every slice costs L2 reads only, and no counters in memory that a
-// caller would have to keep or clear. Biased tokens are few: each is marked in its counter, left out of the
-// pass, and finished by the thread that marked it first, which adds its biases up in the list's order.
+// while they fly (whole numbers: the order of the atomics does not matter), then stores every logit, masked,
+// in vectors, and goes back to the few that the history or a bias changes: done in the vectors' own code
+// they cost a division's instructions for nearly every warp. Reading the history again for every slice costs
+// L2 reads only, and no counters in memory that a caller would have to keep or clear. A biased token is
+// finished by the thread that marked it first.
 #include "common.cuh"
 
 namespace tread {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kCtas = 4;         // CTAs of an SM
 constexpr int kVec = 8;          // consecutive logits of a thread
 constexpr int kMaxBias = 8192;   // 32 bits of ownership a thread
 
@@ -66,19 +68,40 @@ __device__ __forceinline__ void store8(void* out, long long i, const float (&x)[
   }
 }
 
+// element e of a vector held in registers
+template <typename T>
+__device__ __forceinline__ float pick(const int4 (&x)[kVec * sizeof(T) / 16], int e) {
+  constexpr int kPer = 4 / sizeof(T);  // elements of a word
+  const int w = e / kPer;
+  unsigned word = 0;
+#pragma unroll
+  for (int j = 0; j < (int)(kVec * sizeof(T) / 4); ++j) {
+    const int4& q = x[j / 4];
+    const unsigned y = j % 4 == 0 ? q.x : j % 4 == 1 ? q.y : j % 4 == 2 ? q.z : q.w;
+    if (w == j) word = y;
+  }
+  if constexpr (kPer == 2) {
+    const unsigned short h = (unsigned short)(e & 1 ? word >> 16 : word);
+    return Num<T>::to_f(*reinterpret_cast<const T*>(&h));
+  } else {
+    return __uint_as_float(word);
+  }
+}
+
 // VECS: vectors of kVec logits that a thread holds; a slice has VECS * kThreads of them at most
 template <typename T, typename W, int VECS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kCtas)
     adjust_logits_kernel(const __grid_constant__ LogitsArgs a, int slice) {
   using C = Counter<W>;
   extern __shared__ __align__(16) unsigned char s_mem[];
+  __shared__ int s_twice;                  // some token of the slice has more than one bias
   W* count = reinterpret_cast<W*>(s_mem);  // of tokens first - kVec .. first + slice - 1
   const int b = blockIdx.y;
   const T* row = static_cast<const T*>(a.logits) + b * a.ld;
   const long long out_row = b * a.ld_out;
   // vectors start where the row's address is a multiple of 16 bytes: the first slice has the tokens before
   const int head = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
-  const int first = head + blockIdx.x * slice;               // token of the slice's first vector
+  const int first = head + blockIdx.x * slice;  // token of the slice's first vector
   const int begin = blockIdx.x == 0 ? 0 : first;
   const int end = min(a.V, first + slice);
   if (begin >= end) return;
@@ -96,13 +119,14 @@ __global__ void __launch_bounds__(kThreads)
   const int origin = first - kVec;
   for (int i = threadIdx.x; i < (int)((slice + kVec) * sizeof(W) / 16); i += kThreads)
     reinterpret_cast<int4*>(s_mem)[i] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0) s_twice = 0;
   __syncthreads();
   if (a.tokens) {
     long long len = a.lens ? a.lens[b] : a.max_tokens;
     len = len < 0 ? 0 : len > a.max_tokens ? a.max_tokens : len;
     const long long prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
     const long long* ids = reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_ld;
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 4;
     for (int i0 = threadIdx.x; i0 < (int)len; i0 += kThreads * kAhead) {
       long long v[kAhead];
 #pragma unroll
@@ -119,15 +143,21 @@ __global__ void __launch_bounds__(kThreads)
   }
   unsigned mine = 0;  // biases whose token this thread marked first
   const int64_t* bias_ids = a.bias_ids + b * a.bias_ids_ld;
+  const float* bias = a.bias + b * a.bias_ld;
   for (int i = threadIdx.x, k = 0; i < a.num_bias; i += kThreads, ++k) {
     const long long v = bias_ids[i];
-    if (v >= begin && v < end && !(C::mark(count, (int)v - origin, C::kBiased) & C::kBiased)) mine |= 1u << k;
+    if (v < begin || v >= end) continue;
+    if (C::mark(count, (int)v - origin, C::kBiased) & C::kBiased)
+      s_twice = 1;
+    else
+      mine |= 1u << k;
   }
   __syncthreads();
   const float rep = a.repetition ? a.repetition[b] : a.repetition_all;
   const float pres = a.presence ? a.presence[b] : a.presence_all;
   const float freq = a.frequency ? a.frequency[b] : a.frequency_all;
   const unsigned* allowed = a.allowed ? reinterpret_cast<const unsigned*>(a.allowed) + b * a.allowed_ld : nullptr;
+  auto is_allowed = [&](int v) { return !allowed || (allowed[v >> 5] >> (v & 31)) & 1; };
   auto penalised = [&](float f, unsigned c) {
     if (c & ~C::kBiased) {
       f = f > 0.f ? f / rep : f * rep;
@@ -135,25 +165,6 @@ __global__ void __launch_bounds__(kThreads)
     }
     return f;
   };
-  auto single = [&](int v) {  // one token, if it has no bias
-    const unsigned c = count[v - origin];
-    if (c & C::kBiased) return;
-    float f = penalised(Num<T>::to_f(row[v]), c);
-    if (allowed && !((allowed[v >> 5] >> (v & 31)) & 1)) f = -INFINITY;
-    store(a.out, out_row + v, a.out_dtype, f);
-  };
-  for (int k = 0; k < 32 && (mine >> k); ++k) {
-    if (!((mine >> k) & 1)) continue;
-    const long long v = bias_ids[k * kThreads + threadIdx.x];
-    float sum = 0.f;
-    for (int j = 0; j < a.num_bias; ++j)
-      if (bias_ids[j] == v) sum += a.bias[b * a.bias_ld + j];
-    float f = penalised(Num<T>::to_f(row[v]), count[v - origin]) + sum;
-    if (allowed && !((allowed[v >> 5] >> (v & 31)) & 1)) f = -INFINITY;
-    store(a.out, out_row + v, a.out_dtype, f);
-  }
-  if (threadIdx.x < first - begin && threadIdx.x < end) single(threadIdx.x);  // the first slice's tokens before
-  if (threadIdx.x < end - first - vecs * kVec) single(first + vecs * kVec + threadIdx.x);
   const bool aligned =
       (reinterpret_cast<uintptr_t>(a.out) + (out_row + first) * (a.out_dtype == TREAD_F32 ? 4 : 2)) % 16 == 0;
 #pragma unroll
@@ -168,34 +179,18 @@ __global__ void __launch_bounds__(kThreads)
       u.raw = x[k][e * sizeof(T) / 16];
       f[e] = Num<T>::to_f(u.e[e % (16 / sizeof(T))]);
     }
-    unsigned biased = 0;
-    const int4* c = reinterpret_cast<const int4*>(count + (i + 1) * kVec);
-    unsigned w[sizeof(W) * 2];
-#pragma unroll
-    for (int j = 0; j < (int)sizeof(W) / 2; ++j) *reinterpret_cast<int4*>(w + 4 * j) = c[j];
-    unsigned any = 0;
-#pragma unroll
-    for (int j = 0; j < (int)sizeof(W) * 2; ++j) any |= w[j];
-    if (any) {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const unsigned n = sizeof(W) == 4 ? w[e % (sizeof(W) * 2)] : (w[e / 2] >> ((e & 1) * 16)) & 0xffffu;
-        f[e] = penalised(f[e], n);
-        if (n & C::kBiased) biased |= 1u << e;
-      }
-    }
+    unsigned bits = 0xff;
     if (allowed) {
       const int shift = v & 31;
-      unsigned bits = allowed[v >> 5] >> shift;
+      bits = allowed[v >> 5] >> shift;
       if (shift > 32 - kVec) bits |= allowed[(v >> 5) + 1] << (32 - shift);
 #pragma unroll
       for (int e = 0; e < kVec; ++e)
         if (!((bits >> e) & 1)) f[e] = -INFINITY;
     }
-    if (biased || !aligned) {
+    if (!aligned) {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        if (!((biased >> e) & 1)) store(a.out, out_row + v + e, a.out_dtype, f[e]);
+      for (int e = 0; e < kVec; ++e) store(a.out, out_row + v + e, a.out_dtype, f[e]);
     } else if (a.out_dtype == TREAD_F32) {
       store8<float>(a.out, out_row + v, f);
     } else if (a.out_dtype == TREAD_BF16) {
@@ -203,18 +198,69 @@ __global__ void __launch_bounds__(kThreads)
     } else {
       store8<__half>(a.out, out_row + v, f);
     }
+    // which of them the history changes: those again (a biased token is another thread's)
+    const W* c = count + (i + 1) * kVec;
+    unsigned changed = 0;
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(W) / 2; ++j) {
+      const int4 q = reinterpret_cast<const int4*>(c)[j];
+      if (q.x | q.y | q.z | q.w) {
+#pragma unroll
+        for (int e = 0; e < 16 / (int)sizeof(W); ++e) {
+          const unsigned w = e * sizeof(W) / 4 == 0 ? q.x : e * sizeof(W) / 4 == 1 ? q.y : e * sizeof(W) / 4 == 2 ? q.z : q.w;
+          const unsigned n = sizeof(W) == 4 ? w : (w >> ((e & 1) * 16)) & 0xffffu;
+          if (n && !(n & C::kBiased)) changed |= 1u << (j * (16 / sizeof(W)) + e);
+        }
+      }
+    }
+    changed &= bits;
+    while (changed) {
+      const int e = __ffs(changed) - 1;
+      changed &= changed - 1;
+      store(a.out, out_row + v + e, a.out_dtype, penalised(pick<T>(x[k], e), c[e]));
+    }
+  }
+  auto single = [&](int v) {
+    const unsigned c = count[v - origin];
+    if (c & C::kBiased) return;
+    const float f = Num<T>::to_f(row[v]);
+    store(a.out, out_row + v, a.out_dtype, is_allowed(v) ? penalised(f, c) : -INFINITY);
+  };
+  // the first slice's tokens before its vectors (a short row may have no others), and the row's last ones
+  const int tid = threadIdx.x;
+  if (tid < min(first, end) - begin) single(begin + tid);
+  if (tid < end - first - vecs * kVec) single(first + vecs * kVec + tid);
+  if (a.num_bias) {
+    // behind the vectors' stores; where out is logits, an allowed token still has its logit
+    __syncthreads();
+    for (int k = 0; k < 32 && (mine >> k); ++k) {
+      if (!((mine >> k) & 1)) continue;
+      const int i = k * kThreads + threadIdx.x;
+      const int v = (int)bias_ids[i];
+      float sum = bias[i];
+      if (s_twice) {
+        sum = 0.f;
+        for (int j = 0; j < a.num_bias; ++j)
+          if (bias_ids[j] == v) sum += bias[j];
+      }
+      store(a.out, out_row + v, a.out_dtype,
+            is_allowed(v) ? penalised(Num<T>::to_f(row[v]), count[v - origin]) + sum : -INFINITY);
+    }
   }
 }
 
 template <typename T, typename W, int VECS>
 int launch(const LogitsArgs& a, cudaStream_t st) {
-  // slices of whole passes of the CTA, as small as leaves about four CTAs per SM
-  const int pass = kThreads * kVec;
-  const long long want = 592 / a.B > 1 ? 592 / a.B : 1;
-  int slice = (int)((a.V + want * pass - 1) / (want * pass)) * pass;
-  if (slice > VECS * pass) slice = VECS * pass;
+  int device = 0, sms = 0;
+  TREAD_CHECK_CUDA(cudaGetDevice(&device));
+  TREAD_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  // equal slices, as many as run at once, down to one vector a thread
+  constexpr int kPass = kThreads * kVec;
+  int slices = sms * kCtas / a.B;
+  const int most = (int)(((long long)a.V + kPass - 1) / kPass), least = (most + VECS - 1) / VECS;
+  slices = slices > most ? most : slices < least ? least : slices;
+  const int slice = (((a.V + slices - 1) / slices) + 63) / 64 * 64;  // whole vectors of counters
   const int smem = (slice + kVec) * (int)sizeof(W);
-  const int slices = (int)(((long long)a.V + slice - 1) / slice);  // the first one has up to kVec - 1 tokens more
   auto kern = adjust_logits_kernel<T, W, VECS>;
   if (smem > 48 * 1024) TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kern<<<dim3(slices, a.B), kThreads, smem, st>>>(a, slice);
@@ -250,8 +296,8 @@ extern "C" int tread_adjust_logits(const tread_adjust_logits_args* args, tread_s
   if (!a.tokens) a.max_tokens = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (a.dtype) {
-    case TREAD_BF16: return dispatch<__nv_bfloat16, 8>(a, st);
-    case TREAD_F16: return dispatch<__half, 8>(a, st);
+    case TREAD_BF16: return dispatch<__nv_bfloat16, 9>(a, st);
+    case TREAD_F16: return dispatch<__half, 9>(a, st);
     default: return dispatch<float, 4>(a, st);
   }
 }
