@@ -163,6 +163,15 @@ def test_many_biases_and_every_row_offset():
         _check(kernels.adjust_logits(f, out=torch.empty(5, V, dtype=HF, device=DEV), **kf), f, **kf)
 
 
+@pytest.mark.parametrize("H", [4000, 5500, 6200, 6600, 7400, 16383, 16384])
+def test_shared_memory_of_every_size(H):
+    """Histories whose lists bring a CTA's shared memory to either side of 48 KB, and both widths of counters."""
+    logits, kw = _case(64, 152064, H, BF, H)
+    few = slice(0, 2)
+    got = kernels.adjust_logits(logits, **kw)
+    _check(got[few], logits[few], **{k: v[few] for k, v in kw.items()})
+
+
 def test_graph_replay_and_streams():
     logits, kw = _case(4, 20000, 100, BF, 14)
     want = kernels.adjust_logits(logits, **kw)

@@ -261,7 +261,7 @@ int launch(const LogitsArgs& a, cudaStream_t st) {
   const int slice = (((a.V + slices - 1) / slices) + 63) / 64 * 64;  // whole vectors of counters
   const int smem = (slice + kVec) * (int)sizeof(W) + (slice < a.max_tokens ? slice : a.max_tokens) * 2 + kVec * 2;
   auto kern = adjust_logits_kernel<T, W, VECS>;
-  if (smem > 48 * 1024) TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 32 * 1024) TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kern<<<dim3(slices, a.B), kThreads, smem, st>>>(a, slice);
   TREAD_CHECK_LAUNCH("adjust_logits_kernel");
   return TREAD_OK;
@@ -287,7 +287,7 @@ extern "C" int tread_adjust_logits(const tread_adjust_logits_args* args, tread_s
   TREAD_CHECK_ARG(dtype_size(a.dtype) != 0 && dtype_size(a.out_dtype) != 0, "adjust_logits: unknown dtype %d or %d",
                   a.dtype, a.out_dtype);
   TREAD_CHECK_ARG(a.B == 1 || (a.ld >= a.V && a.ld_out >= a.V), "adjust_logits: row stride below the vocabulary");
-  TREAD_CHECK_ARG(a.max_tokens >= 0 && (!a.tokens || a.B == 1 || a.tokens_ld >= a.max_tokens),
+  TREAD_CHECK_ARG(a.max_tokens >= 0 && a.max_tokens <= (1 << 30) && (!a.tokens || a.B == 1 || a.tokens_ld >= a.max_tokens),
                   "adjust_logits: bad history");
   TREAD_CHECK_ARG(a.num_bias <= kMaxBias, "adjust_logits: more than %d biases", kMaxBias);
   TREAD_CHECK_ARG(a.num_bias >= 0 && (a.num_bias == 0 || (a.bias_ids && a.bias)), "adjust_logits: bad biases");
@@ -295,8 +295,8 @@ extern "C" int tread_adjust_logits(const tread_adjust_logits_args* args, tread_s
   if (!a.tokens) a.max_tokens = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (a.dtype) {
-    case TREAD_BF16: return dispatch<__nv_bfloat16, 8>(a, st);
-    case TREAD_F16: return dispatch<__half, 8>(a, st);
-    default: return dispatch<float, 4>(a, st);
+    case TREAD_BF16: return dispatch<__nv_bfloat16, 4>(a, st);
+    case TREAD_F16: return dispatch<__half, 4>(a, st);
+    default: return dispatch<float, 2>(a, st);
   }
 }
