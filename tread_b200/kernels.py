@@ -474,22 +474,27 @@ def rows_gemm(x, w, bias=None, out=None, accumulate=False, err=None, stream=None
 
 # ---- decode step over a paged cache ---------------------------------------------------------------
 
+# The checks of these wrappers read each shape and stride once and compare device numbers: a decode step
+# makes two such calls a layer, and host time is what bounds it for few sequences.
+
 def _pages(k_pages, v_pages):
-    """(page stride, head stride) of a pair of pools [N, Hkv, page_size, D] with contiguous
+    """(shape, page stride, head stride) of a pair of pools [N, Hkv, page_size, D] with contiguous
     [page_size, D] planes: a whole pool, or one layer of [N, L, Hkv, page_size, D]."""
     C.require_cuda(k_pages, "k_pages")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+    shape, stride = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != stride:
         raise ValueError("k_pages and v_pages must be [pages, Hkv, page_size, D] of one shape and strides")
-    sp, sh, st, sd = k_pages.stride()
-    if (sd != 1 and k_pages.shape[3] != 1) or st != k_pages.shape[3] or k_pages.dtype != v_pages.dtype:
+    if (stride[3] != 1 or (stride[2] != shape[3] and shape[2] != 1)) or k_pages.dtype != v_pages.dtype:
         raise ValueError("k_pages and v_pages must share a dtype and have contiguous [page_size, D] planes")
-    return sp, sh
+    return shape, stride[0], stride[1]
 
 
-def _table(table, name="table"):
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
-        raise ValueError(f"{name} must be int32 [sequences, pages] with unit column stride")
-    return table.stride(0)
+def _table(table):
+    """(row stride, sequences, pages of a sequence) of a page table."""
+    shape, stride = table.shape, table.stride()
+    if len(shape) != 2 or table.dtype != torch.int32 or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError("table must be int32 [sequences, pages] with unit column stride")
+    return stride[0], shape[0], shape[1]
 
 
 def _index(t, n, dtype, name):
@@ -497,19 +502,21 @@ def _index(t, n, dtype, name):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of length {n}")
 
 
-def _elsewhere(device, stream):
-    """The context in which a call on tensors of `device` has to run, or None where it is the current
-    one: launches and allocations go to the current device and stream."""
+def _elsewhere(index, stream):
+    """The context in which a call on tensors of CUDA device `index` has to run, or None where it is the
+    current one: launches and allocations go to the current device and stream."""
     if stream is not None:
-        if stream.device != device:
-            raise ValueError(f"the stream is on {stream.device}, the call's tensors on {device}")
+        if stream.device.index != index:
+            raise ValueError(f"the stream is on {stream.device}, the call's tensors on cuda:{index}")
         return torch.cuda.stream(stream)
-    return None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+    return None if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
-def _launch(fn, name, device, args):
-    """Call the library's fn(args struct, current stream)."""
-    C.check(fn(args, torch._C._cuda_getCurrentRawStream(device.index)), name)
+def _launch(name, index, args):
+    """Call the library's function `name` with its argument struct on the current stream of a device."""
+    rc = getattr(C.lib(), name)(args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        C.check(rc, name)
 
 
 def _ptr(t):
@@ -532,21 +539,22 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
     err: device error word; a row whose sequence, position or page is out of range appends nothing, gets
       a zero query and sets bit 0.
     Returns the rotated queries [R, Hq, D] (q_out, which may be q itself), or None without q."""
-    sp, sh = _pages(k_pages, v_pages)
-    device = k_pages.device
-    other = _elsewhere(device, stream)
+    (N, Hkv, page_size, D), sp, sh = _pages(k_pages, v_pages)
+    index = k_pages.get_device()
+    other = _elsewhere(index, stream)
     if other is not None:
         with other:
             return paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out, err)
-    N, Hkv, page_size, D = k_pages.shape
-    C.same_device(k_pages, k=k, v=v, v_pages=v_pages, table=table, pos=pos, seq=seq, inv_freq=inv_freq,
-                  rope_pos=rope_pos, q=q, q_out=q_out, err=err)
-    if k.dim() != 3 or k.shape[1:] != (Hkv, D) or k.stride(2) != 1 or v.shape != k.shape or v.stride(2) != 1:
+    if not (k.get_device() == v.get_device() == v_pages.get_device() == table.get_device() == pos.get_device() == index):
+        C.same_device(k_pages, k=k, v=v, v_pages=v_pages, table=table, pos=pos)
+    dtype, shape = k.dtype, k.shape
+    k_stride, v_stride = k.stride(), v.stride()
+    if len(shape) != 3 or shape[1] != Hkv or shape[2] != D or v.shape != shape or k_stride[2] != 1 or v_stride[2] != 1:
         raise ValueError(f"k and v must be [R, {Hkv}, {D}] with unit last stride")
-    R = k.shape[0]
-    if not (k.dtype == v.dtype == k_pages.dtype):
+    if not (dtype == v.dtype == k_pages.dtype):
         raise TypeError("k, v and the pages must share a dtype")
-    ld, (S, width) = _table(table), table.shape
+    R = shape[0]
+    ld, S, width = _table(table)
     _index(pos, R, torch.int64, "pos")
     if seq is not None:
         _index(seq, R, torch.int32, "seq")
@@ -561,21 +569,23 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
         if q_out is not None:
             raise ValueError("q_out without q")
     else:
-        if q.dim() != 3 or q.shape[0] != R or q.shape[2] != D or q.stride(2) != 1 or q.dtype != k.dtype:
+        shape, q_stride = q.shape, q.stride()
+        if len(shape) != 3 or shape[0] != R or shape[2] != D or q_stride[2] != 1 or q.dtype != dtype:
             raise ValueError(f"q must be [{R}, Hq, {D}] of k's dtype with unit last stride")
         if inv_freq is None:
             raise ValueError("q without inv_freq: nothing rotates it")
-        Hq, q_ld, q_sh = q.shape[1], q.stride(0), q.stride(1)
+        Hq, q_ld, q_sh = shape[1], q_stride[0], q_stride[1]
         if q_out is None:
-            q_out = torch.empty((R, Hq, D), dtype=q.dtype, device=device)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
-            raise ValueError(f"q_out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
-    k_ld, k_sh, _ = k.stride()
-    v_ld, v_sh, _ = v.stride()
-    _launch(C.lib().tread_paged_append, "tread_paged_append", device, C.PAGED_APPEND.pack(
+            q_out = q.new_empty(shape)
+        elif q_out.shape != shape or q_out.dtype != dtype or not q_out.is_contiguous():
+            raise ValueError(f"q_out must be a contiguous {tuple(shape)} tensor of q's dtype")
+    for t in (seq, rope_pos, inv_freq, q, q_out, err):
+        if t is not None and t.get_device() != index:
+            C.same_device(k_pages, seq=seq, inv_freq=inv_freq, rope_pos=rope_pos, q=q, q_out=q_out, err=err)
+    _launch("tread_paged_append", index, C.PAGED_APPEND.pack(
         k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
-        _ptr(seq), pos.data_ptr(), _ptr(rope_pos), _ptr(inv_freq), _ptr(err), k_ld, k_sh, v_ld, v_sh, q_ld, q_sh, sp, sh,
-        N, ld, page_size, S, width, R, Hq, Hkv, D, C.dtype_code(k.dtype), attn_scaling))
+        _ptr(seq), pos.data_ptr(), _ptr(rope_pos), _ptr(inv_freq), _ptr(err), k_stride[0], k_stride[1], v_stride[0],
+        v_stride[1], q_ld, q_sh, sp, sh, N, ld, page_size, S, width, R, Hq, Hkv, D, C.dtype_code(dtype), attn_scaling))
     return q_out
 
 
@@ -586,42 +596,42 @@ def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=No
     has a score above -inf, or there is none (length 0), the output is zero.
     err: device error word; a length that the table has no pages for gives a row of zeros and sets bit
     1, and so does a page id outside the pool, whose keys count as masked. Returns out [B, Hq, D]."""
-    sp, sh = _pages(k_pages, v_pages)
-    device = k_pages.device
-    other = _elsewhere(device, stream)
+    (N, Hkv, page_size, D), sp, sh = _pages(k_pages, v_pages)
+    index = k_pages.get_device()
+    other = _elsewhere(index, stream)
     if other is not None:
         with other:
             return paged_attn(q, k_pages, v_pages, table, lens, out, sm_scale, err)
-    N, Hkv, page_size, D = k_pages.shape
-    C.same_device(k_pages, q=q, v_pages=v_pages, table=table, lens=lens, out=out, err=err)
-    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != D) or (
-            q.dtype != k_pages.dtype):
+    if not (q.get_device() == v_pages.get_device() == table.get_device() == lens.get_device() == index) or (
+            out is not None or err is not None):
+        C.same_device(k_pages, q=q, v_pages=v_pages, table=table, lens=lens, out=out, err=err)
+    shape, stride, dtype = q.shape, q.stride(), q.dtype
+    if len(shape) != 3 or shape[2] != D or stride[2] != 1 or (shape[1] > 1 and stride[1] != D) or dtype != k_pages.dtype:
         raise ValueError(f"q must be [B, Hq, {D}] of the pages' dtype with contiguous rows")
-    B, Hq, _ = q.shape
-    ld, (rows, width) = _table(table), table.shape
-    if rows != B:
+    B, Hq, _ = shape
+    ld, S, width = _table(table)
+    if S != B:
         raise ValueError(f"table must have a row for each of the {B} sequences")
     _index(lens, B, torch.int64, "lens")
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=q.dtype, device=device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
-    lib = C.lib()
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != dtype or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {tuple(shape)} tensor of q's dtype")
     # one workspace a call, from the allocator: calls of several streams, threads and graphs share none
-    nbytes = lib.tread_paged_attn_workspace_bytes(Hq, Hkv, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _launch(lib.tread_paged_attn, "tread_paged_attn", device, C.PAGED_ATTN.pack(
+    nbytes = C.lib().tread_paged_attn_workspace_bytes(Hq, Hkv, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _launch("tread_paged_attn", index, C.PAGED_ATTN.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), _ptr(err),
-        ws.data_ptr(), q.stride(0), sp, sh, N, ld, nbytes, page_size, width, B, Hq, Hkv, D, C.dtype_code(q.dtype),
+        ws.data_ptr(), stride[0], sp, sh, N, ld, nbytes, page_size, width, B, Hq, Hkv, D, C.dtype_code(dtype),
         D ** -0.5 if sm_scale is None else sm_scale))
     return out
 
 
-def _per_row(x, B, name, device):
-    """A penalty as (device pointer or None, value for all rows)."""
+def _per_row(x, B, name, index):
+    """A penalty as (device pointer or 0, value for all rows)."""
     if isinstance(x, torch.Tensor):
-        if x.device != device:
-            raise ValueError(f"{name} is on {x.device}, the logits on {device}")
+        if x.get_device() != index:
+            raise ValueError(f"{name} is on {x.device}, the logits on cuda:{index}")
         _index(x, B, torch.float32, name)
         return x.data_ptr(), 1.0
     return 0, float(x)
@@ -629,10 +639,10 @@ def _per_row(x, B, name, device):
 
 def _by_row(t, B, width, dtype, name):
     """Row stride of t [B, width], or 0 for one row [width] that serves every row."""
-    if t.dtype != dtype or t.dim() not in (1, 2) or t.shape[-1] != width or (width > 1 and t.stride(-1) != 1) or (
-            t.dim() == 2 and t.shape[0] != B):
+    shape, stride = t.shape, t.stride()
+    if t.dtype != dtype or not (shape == (B, width) or shape == (width,)) or (width > 1 and stride[-1] != 1):
         raise ValueError(f"{name} must be {dtype} [{B}, {width}] or [{width}] with unit last stride")
-    return t.stride(0) if t.dim() == 2 else 0
+    return stride[0] if len(shape) == 2 else 0
 
 
 def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1.0, presence=0.0, frequency=0.0,
@@ -651,31 +661,36 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
       [W] for all rows, W = ceil(V / 32)) is 0.
     Returns out: fp32 [B, V] by default; a given one may be of any supported dtype, or logits itself."""
     C.require_cuda(logits, "logits")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("logits must be [B, V] with unit column stride")
-    device = logits.device
-    other = _elsewhere(device, stream)
+    index = logits.get_device()
+    other = _elsewhere(index, stream)
     if other is not None:
         with other:
             return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
                                  allowed, out)
-    B, V = logits.shape
-    C.same_device(logits, tokens=tokens, lens=lens, prompt_lens=prompt_lens, bias_ids=bias_ids, bias=bias,
-                  allowed=allowed, out=out)
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
+        raise ValueError("logits must be [B, V] with unit column stride")
+    B, V = shape
+    for t in (tokens, lens, prompt_lens, bias_ids, bias, allowed, out):
+        if t is not None and t.get_device() != index:
+            C.same_device(logits, tokens=tokens, lens=lens, prompt_lens=prompt_lens, bias_ids=bias_ids, bias=bias,
+                          allowed=allowed, out=out)
     H = tok_ld = 0
     if tokens is not None:
-        if tokens.dim() != 2 or tokens.shape[0] != B or tokens.dtype != torch.int64 or (
-                tokens.shape[1] > 1 and tokens.stride(1) != 1):
+        t_shape, t_stride = tokens.shape, tokens.stride()
+        if len(t_shape) != 2 or t_shape[0] != B or tokens.dtype != torch.int64 or (t_shape[1] > 1 and t_stride[1] != 1):
             raise ValueError(f"tokens must be int64 [{B}, H] with unit column stride")
-        H, tok_ld = tokens.shape[1], tokens.stride(0)
-    for t, name in ((lens, "lens"), (prompt_lens, "prompt_lens")):
-        if t is not None:
-            if tokens is None:
-                raise ValueError(f"{name} without tokens")
-            _index(t, B, torch.int64, name)
-    rep, pres, freq = (_per_row(x, B, n, device) for x, n in ((repetition, "repetition"), (presence, "presence"),
-                                                              (frequency, "frequency")))
-    if not rep[1] > 0:
+        H, tok_ld = t_shape[1], t_stride[0]
+        if lens is not None:
+            _index(lens, B, torch.int64, "lens")
+        if prompt_lens is not None:
+            _index(prompt_lens, B, torch.int64, "prompt_lens")
+    elif lens is not None or prompt_lens is not None:
+        raise ValueError("lens and prompt_lens without tokens")
+    rep, rep_all = _per_row(repetition, B, "repetition", index)
+    pres, pres_all = _per_row(presence, B, "presence", index)
+    freq, freq_all = _per_row(frequency, B, "frequency", index)
+    if not rep_all > 0:
         raise ValueError(f"repetition must be above 0, got {repetition}")
     nb = ids_ld = bias_ld = 0
     if (bias is None) != (bias_ids is None):
@@ -685,15 +700,18 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
         ids_ld, bias_ld = _by_row(bias_ids, B, nb, torch.int64, "bias_ids"), _by_row(bias, B, nb, torch.float32, "bias")
     allowed_ld = 0 if allowed is None else _by_row(allowed, B, (V + 31) // 32, torch.int32, "allowed")
     if out is None:
-        out = torch.empty((B, V), dtype=torch.float32, device=device)
-    elif out.shape != (B, V) or (V > 1 and out.stride(1) != 1):
-        raise ValueError(f"out must be [{B}, {V}] with unit column stride")
-    elif out.data_ptr() == logits.data_ptr() and (out.dtype != logits.dtype or out.stride(0) != logits.stride(0)):
-        raise ValueError("out over logits must have their dtype and row stride")
-    _launch(C.lib().tread_adjust_logits, "tread_adjust_logits", device, C.ADJUST_LOGITS.pack(
-        logits.data_ptr(), out.data_ptr(), _ptr(tokens), _ptr(lens), _ptr(prompt_lens), rep[0], pres[0], freq[0],
-        _ptr(bias_ids), _ptr(bias), _ptr(allowed), logits.stride(0), out.stride(0), tok_ld, ids_ld, bias_ld, allowed_ld, B,
-        V, H, nb, C.dtype_code(logits.dtype), C.dtype_code(out.dtype), rep[1], pres[1], freq[1]))
+        out = torch.empty(shape, dtype=torch.float32, device=logits.device)
+        out_ld = V
+    else:
+        out_ld, *last = out.stride()
+        if out.shape != shape or (V > 1 and last != [1]):
+            raise ValueError(f"out must be [{B}, {V}] with unit column stride")
+        if out.data_ptr() == logits.data_ptr() and (out.dtype != logits.dtype or out_ld != stride[0]):
+            raise ValueError("out over logits must have their dtype and row stride")
+    _launch("tread_adjust_logits", index, C.ADJUST_LOGITS.pack(
+        logits.data_ptr(), out.data_ptr(), _ptr(tokens), _ptr(lens), _ptr(prompt_lens), rep, pres, freq, _ptr(bias_ids),
+        _ptr(bias), _ptr(allowed), stride[0], out_ld, tok_ld, ids_ld, bias_ld, allowed_ld, B, V, H, nb,
+        C.dtype_code(logits.dtype), C.dtype_code(out.dtype), rep_all, pres_all, freq_all))
     return out
 
 
