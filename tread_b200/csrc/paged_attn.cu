@@ -10,7 +10,8 @@
 //
 // Split. The lengths are on the device, so the kernel itself deals out the work: all sequences' keys, per
 // KV head in units of 16, form one line that is cut into equal shares, one per CTA, whatever the lengths.
-// A CTA's share covers parts of one or more items (sequence, KV head). Its warps take the units of the
+// An item costs more than its units (its queries, the joining of the warps, the output): about kItemCost of
+// them, which are counted in. A CTA's share covers parts of one or more items (sequence, KV head). Its warps take the units of the
 // share in turn, each with a ring of units in flight in shared memory (cp.async, 16 bytes a lane, rows
 // swizzled so that eight rows' same chunk lie in eight banks), its own running maximum and sum, and its
 // own accumulators. At an item's end the warps' states are joined in shared memory; an item that several
@@ -31,6 +32,8 @@ namespace {
 
 constexpr int kUnit = 16;      // keys of one unit
 constexpr int kMaxCtas = 384;  // shares at most
+constexpr int kItemCost = 4;   // units that an item's fixed cost amounts to
+constexpr int kMinShare = 4;   // a unit for every warp: more parts cost more to join
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // the running maximum may lag by 2^8: weights stay far inside fp16's range
 
@@ -402,54 +405,72 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ unsigned s_live[W][kStages];
   __shared__ float2 s_ml[W][GP];
-  __shared__ long long s_scan[kThreads / 32];
+  __shared__ long long s_scan[W], s_ends[2];
+  __shared__ int s_items[W];
   __shared__ Place s_place;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* s_o = reinterpret_cast<float*>(smem + kStages * W * S::kUnitBytes);
   void* extra = smem + kStages * W * S::kUnitBytes + S::kJoin;
   const unsigned ring = smem_addr(smem) + warp * (kStages * S::kUnitBytes);
 
-  // the line: every thread adds up a run of sequences, a scan places the runs
+  // the line: every thread adds up a run of sequences, a scan places the runs. Units and items are summed side
+  // by side (a sequence has under 2^27 units; 2^32 sequences there are not).
   const int run = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(a.B, (int)threadIdx.x * run), b1 = min(a.B, b0 + run);
-  long long mine = 0;
+  long long units = 0;
+  int items = 0;
   for (int b = b0; b < b1; ++b) {
     const int len = length_of(a, b);
-    mine += units_of(len);
+    units += units_of(len);
+    items += len > 0;
     if (len == 0 && b % gridDim.x == blockIdx.x) {
       const long long n = __ldg(reinterpret_cast<const long long*>(a.lens) + b);
       if (n != 0 && a.err) atomicOr(a.err, 2u);
     }
   }
-  long long upto = mine;
+  long long upto = units;
+  int upto_items = items;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const long long x = __shfl_up_sync(0xffffffffu, upto, off);
-    if (lane >= off) upto += x;
+    const int y = __shfl_up_sync(0xffffffffu, upto_items, off);
+    if (lane >= off) upto += x, upto_items += y;
   }
-  if (lane == 31) s_scan[warp] = upto;
-  if (threadIdx.x == 0) s_place.b = -1;
+  if (lane == 31) s_scan[warp] = upto, s_items[warp] = upto_items;
   __syncthreads();
-  long long before = upto - mine, total = 0;
+  long long before = upto - units, total = 0;
+  int before_items = upto_items - items, total_items = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
+    if (w < warp) before += s_scan[w], before_items += s_items[w];
+    total += s_scan[w], total_items += s_items[w];
   }
-  total *= a.Hkv;
-  long long share = (total + gridDim.x - 1) / gridDim.x;
-  if (share < W) share = W;  // a unit for every warp at least: more parts cost more to join
-  const long long u0 = blockIdx.x * share, u1 = min(total, u0 + share);
-  if (u0 < u1 && u0 >= before * a.Hkv && u0 < (before + mine) * a.Hkv) {
-    long long at = before * a.Hkv;
+  const long long line = (total + (long long)kItemCost * total_items) * a.Hkv;
+  long long share = (line + gridDim.x - 1) / gridDim.x;
+  if (share < kMinShare) share = kMinShare;
+  // the share's ends on the line of units alone, and the place of its first unit
+  const long long c0 = min(line, blockIdx.x * share), c1 = min(line, c0 + share);
+  const long long run0 = (before + (long long)kItemCost * before_items) * a.Hkv;
+  const long long run1 = run0 + (units + (long long)kItemCost * items) * a.Hkv;
+  if (threadIdx.x == 0) s_ends[0] = s_ends[1] = total * a.Hkv;  // of a cut at the line's end
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    __syncthreads();
+    const long long cut = i == 0 ? c0 : c1;
+    if (cut < run0 || cut >= run1) continue;
+    long long at = run0, at_units = before * a.Hkv;
     for (int b = b0;; ++b) {
       const int len = length_of(a, b), n = units_of(len);
-      if (u0 < at + (long long)n * a.Hkv) {
-        const int in = (int)(u0 - at);
-        s_place = Place{b, in / n, in % n, n, len};
+      const long long here = len > 0 ? (long long)(n + kItemCost) * a.Hkv : 0;
+      if (cut < at + here) {
+        const long long in = cut - at;
+        const int g = (int)(in / (n + kItemCost)), j = max(0, (int)(in % (n + kItemCost)) - kItemCost);
+        s_ends[i] = at_units + (long long)g * n + j;
+        if (i == 0) s_place = Place{b, g, j, n, len};
         break;
       }
-      at += (long long)n * a.Hkv;
+      at += here;
+      at_units += (long long)n * a.Hkv;
     }
   }
   // sequences without a key: zeros
@@ -458,6 +479,7 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
       for (int i = threadIdx.x; i < a.Hq * D; i += kThreads)
         static_cast<T*>(a.out)[(long long)b * a.Hq * D + i] = Num<T>::from_f(0.f);
   __syncthreads();
+  const long long u0 = s_ends[0], u1 = s_ends[1];
   if (u0 >= u1) {
     if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
@@ -565,7 +587,7 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
       }
     }
     if (!whole && at.j == 0)  // starts here, ends in the CTA of its last unit
-      open = make_int4((int)((pos + at.n - 1) / share - blockIdx.x + 1), at.b, at.g, slot);
+      open = make_int4((int)((c1 + at.n - seg - 1) / share - blockIdx.x + 1), at.b, at.g, slot);
     pos += seg;
     at.j += seg;
     if (pos < u1) at.settle(a);
@@ -576,55 +598,76 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
 }
 
 // Items whose keys several CTAs share: CTA (c, h) joins head h of the item that starts in share c and
-// ends in another. Its four warps take the parts in turn.
-constexpr int kJoinWarps = 4;
+// ends in another. All parts' maxima and sums are read at once and turned into weights; the warps then take
+// the accumulators in turn, kAhead loads in flight each.
+constexpr int kJoinWarps = 8;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const __grid_constant__ DecodeArgs a) {
-  constexpr int kPer = D / 32;
-  __shared__ float s_o[kJoinWarps][D], s_l[kJoinWarps], s_m[kJoinWarps];
+  constexpr int kPer = D / 32, kAhead = 8, kThreads = kJoinWarps * 32;
+  __shared__ float s_o[kJoinWarps][D], s_m[kJoinWarps], s_l[kJoinWarps], s_f[kMaxCtas];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 open = a.desc[blockIdx.x];
   if (open.x == 0) return;
   const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto state = [&](int i) { return ((blockIdx.x + i) * 2LL + (i == 0 ? open.w : 0)) * a.G + h; };
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < open.x; i += kJoinWarps * 32) top = fmaxf(top, a.ml[state(i)].x);
+  float o[kPer] = {};
+  float2 ml[(kMaxCtas + kThreads - 1) / kThreads];
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < (kMaxCtas + kThreads - 1) / kThreads; ++k) {
+    const int i = threadIdx.x + k * kThreads;
+    ml[k] = i < open.x ? a.ml[state(i)] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[k].x);
+  }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   if (lane == 0) s_m[warp] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_m[w]);
-  float sum = 0.f, o[kPer];
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < open.x; i += kJoinWarps) {
-    const float2 ml = a.ml[state(i)];
-    const float* from = a.part + state(i) * D + lane * kPer;
-    float x[kPer];
-    if constexpr (kPer == 2) {
-      *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from);
-    } else {
+  for (int k = 0; k < (kMaxCtas + kThreads - 1) / kThreads; ++k) {
+    const int i = threadIdx.x + k * kThreads;
+    if (i >= open.x) continue;
+    s_f[i] = weight(ml[k].x, top);
+    sum += s_f[i] * ml[k].y;
+  }
 #pragma unroll
-      for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(x + e) = *reinterpret_cast<const float4*>(from + e);
+  for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if (lane == 0) s_l[warp] = sum;
+  __syncthreads();
+  for (int i0 = warp; i0 < open.x; i0 += kJoinWarps * kAhead) {
+    float x[kAhead][kPer];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kJoinWarps;
+      if (i >= open.x) break;
+      const float* from = a.part + state(i) * D + lane * kPer;
+      if constexpr (kPer == 2) {
+        *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(from);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(x[k] + e) = *reinterpret_cast<const float4*>(from + e);
+      }
     }
-    const float f = weight(ml.x, top);
-    sum += f * ml.y;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] = fmaf(f, x[e], o[e]);
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kJoinWarps;
+      if (i >= open.x) break;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] = fmaf(s_f[i], x[k][e], o[e]);
+    }
   }
 #pragma unroll
   for (int e = 0; e < kPer; ++e) s_o[warp][lane * kPer + e] = o[e];
-  if (lane == 0) s_l[warp] = sum;
   __syncthreads();
   float all = 0.f;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) all += s_l[w];
   const float inv = all == 0.f ? 0.f : 1.f / all;
   T* to = static_cast<T*>(a.out) + ((long long)open.y * a.Hq + open.z * a.G + h) * D;
-  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+  for (int d = threadIdx.x; d < D; d += kThreads) {
     float x = 0.f;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) x += s_o[w][d];
