@@ -12,7 +12,13 @@ timed out waiting for the GPU, 401 bad bearer token) and greedy decoding are the
 so a client of the reference server sees the same API. What differs is below the API: prefill is
 `tread_b200.Engine.prefill` (host token ids in; one host-to-device copy inside the call) and the
 decode steps run the HF model over the `DynamicCache` that prefill hands back, whose layers are
-views of the request's assembled cache.
+views of the request's assembled cache; with `decoder` (a tread_b200.paged.PagedDecoder) they run
+over a paged cache instead, which no token has to copy.
+
+Requests may also carry what the reference has not: repetition_penalty, presence_penalty,
+frequency_penalty, logit_bias ({token id: bias}) and allowed_token_ids (a mask over the vocabulary).
+They change the logits before the greedy choice (tread_b200.kernels.adjust_logits); left at their
+neutral defaults nothing is touched.
 
 The engine is not thread-safe: one lock serialises GPU work; at most `max_queue` requests may be in
 flight. Documents are tokenized as untrusted text (control-token text stays plain text); prefix
@@ -26,6 +32,8 @@ from typing import Annotated
 import torch
 from fastapi import Depends, FastAPI, HTTPException, Request
 from pydantic import BaseModel, Field, StringConstraints
+
+from tread_b200 import kernels
 
 MAX_SEGMENT_CHARS = 200_000
 MAX_DOCUMENTS = 256
@@ -42,6 +50,11 @@ class CompletionRequest(BaseModel):
     max_tokens: int = Field(64, ge=1, le=2048)
     recompute_ratio: float = Field(0.2, ge=0.0, le=1.0)
     policy: str = Field("deviation", pattern="^(deviation|boundary|random)$")
+    repetition_penalty: float = Field(1.0, gt=0.0, le=100.0)
+    presence_penalty: float = Field(0.0, ge=-100.0, le=100.0)
+    frequency_penalty: float = Field(0.0, ge=-100.0, le=100.0)
+    logit_bias: dict[int, Annotated[float, Field(ge=-1e4, le=1e4)]] = Field(default_factory=dict, max_length=1024)
+    allowed_token_ids: list[int] | None = Field(None, min_length=1, max_length=200_000)
 
 
 class _Tokenizer:
@@ -59,9 +72,51 @@ class _Tokenizer:
             return self.tok.decode(ids)
 
 
+class _Adjust:
+    """A request's penalties, biases and mask, applied to its logits step by step; `history` holds the
+    prompt's and the answer's token ids on the device."""
+
+    def __init__(self, req, prompt, vocab, device):
+        ids = list(req.logit_bias) + (req.allowed_token_ids or [])
+        if any(not 0 <= i < vocab for i in ids):
+            raise HTTPException(422, f"logit_bias and allowed_token_ids take token ids from 0 to {vocab - 1}")
+        self.kw = dict(repetition=req.repetition_penalty, presence=req.presence_penalty,
+                       frequency=req.frequency_penalty)
+        if req.logit_bias:
+            self.kw["bias_ids"] = torch.tensor(list(req.logit_bias), dtype=torch.int64, device=device)
+            self.kw["bias"] = torch.tensor(list(req.logit_bias.values()), dtype=torch.float32, device=device)
+        if req.allowed_token_ids is not None:
+            bits = torch.zeros((vocab + 31) // 32 * 32, dtype=torch.int64)
+            bits[torch.tensor(req.allowed_token_ids)] = 1
+            words = (bits.view(-1, 32) << torch.arange(32)).sum(1)
+            self.kw["allowed"] = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32).to(device)
+        n = len(prompt)
+        self.history = torch.zeros(1, n + req.max_tokens, dtype=torch.int64)
+        self.history[0, :n] = torch.tensor(prompt)
+        self.history = self.history.to(device)
+        self.prompt = torch.tensor([n], device=device)
+        self.n = n
+
+    @staticmethod
+    def wanted(req):
+        return (req.repetition_penalty != 1.0 or req.presence_penalty != 0.0 or req.frequency_penalty != 0.0
+                or bool(req.logit_bias) or req.allowed_token_ids is not None)
+
+    def add(self, token):
+        self.history[0, self.n] = token
+        self.n += 1
+
+    def __call__(self, logits):
+        """logits [vocab] -> adjusted fp32 [vocab]."""
+        return kernels.adjust_logits(logits[None], tokens=self.history[:, :self.n], prompt_lens=self.prompt, **self.kw)[0]
+
+
 def build_app(model, tok, engine, eos_ids, max_context=16384, api_key=None, max_queue=16, queue_timeout=30.0,
-              max_seconds=120.0):
-    """FastAPI app serving `engine` (a tread_b200.Engine over `model`) with tokenizer `tok`."""
+              max_seconds=120.0, decoder=None):
+    """FastAPI app serving `engine` (a tread_b200.Engine over `model`) with tokenizer `tok`; `decoder`: a
+    tread_b200.paged.PagedDecoder over the same model to decode with (default: the HF model)."""
+    if decoder is not None and decoder.max_len < max_context:
+        raise ValueError(f"decoder: its pages hold sequences of {decoder.max_len} tokens, max_context is {max_context}")
 
     def auth(request: Request):
         if api_key is not None and not hmac.compare_digest(request.headers.get("authorization", "").encode(),
@@ -89,23 +144,42 @@ def build_app(model, tok, engine, eos_ids, max_context=16384, api_key=None, max_
 
     def generate(req, ids):
         host = [torch.tensor(x, dtype=torch.long) for x in ids]
+        seq = adjust = None
+        if _Adjust.wanted(req):
+            adjust = _Adjust(req, [t for seg in ids for t in seg], model.config.vocab_size, model.device)
+        pick = lambda logits: int((adjust(logits) if adjust else logits).argmax().item())  # noqa: E731
         with torch.inference_mode():
             t0 = time.perf_counter()
             logits, cache, st = engine.prefill(host[0], host[1:-1], host[-1], ratio=req.recompute_ratio,
                                                policy=req.policy, namespace=req.tenant)
-            nxt = int(logits.argmax().item())
+            nxt = pick(logits)
             out, reason = [], "stop"
             dev = logits.device
-            while nxt not in eos:
-                if len(out) >= req.max_tokens:
-                    reason = "length"
-                    break
-                if time.perf_counter() - t0 > max_seconds:
-                    reason = "time"
-                    break
-                out.append(nxt)
-                o = model(torch.tensor([[nxt]], device=dev), past_key_values=cache, use_cache=True, logits_to_keep=1)
-                cache, nxt = o.past_key_values, int(o.logits[0, -1].argmax().item())
+            try:
+                if decoder is not None:
+                    seq = decoder.admit(cache)
+                    cache = None
+                while nxt not in eos:
+                    if len(out) >= req.max_tokens:
+                        reason = "length"
+                        break
+                    if time.perf_counter() - t0 > max_seconds:
+                        reason = "time"
+                        break
+                    out.append(nxt)
+                    if adjust:
+                        adjust.add(nxt)
+                    if decoder is not None:
+                        nxt = pick(decoder.step([seq], [nxt])[0])
+                    else:
+                        o = model(torch.tensor([[nxt]], device=dev), past_key_values=cache, use_cache=True,
+                                  logits_to_keep=1)
+                        cache, nxt = o.past_key_values, pick(o.logits[0, -1])
+                if decoder is not None:
+                    decoder.net.check_errors()
+            finally:
+                if seq is not None:
+                    decoder.release(seq)
             total = time.perf_counter() - t0
         counters["requests"] += 1
         counters["ttft_ms_sum"] += st.t["ttft"] * 1e3
