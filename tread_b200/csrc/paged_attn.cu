@@ -20,8 +20,9 @@
 //
 // 16-bit types run on mma.sync with keys as rows and the group's query heads as the 8 columns, so that a
 // group of 7 fills 7 of 8 columns (heads as rows would fill 7 of 16): S^T = K Q^T, O^T = V^T P^T, and the
-// heads of S^T's, P^T's and O^T's columns stay in the same lanes. P is rounded to the type once before it
-// meets V (its sum stays fp32): half a step of each weight, the size of the output's own rounding.
+// heads of S^T's, P^T's and O^T's columns stay in the same lanes. P meets V as the sum of two numbers of the
+// type, its rounding and what that left out: the weights keep 16 bits or more, and the output's own rounding
+// is all that is lost (rounded once, the weights add as much error again); 1 % of the time.
 // fp32 runs on FMAs.
 #include <type_traits>
 
@@ -41,10 +42,16 @@ struct DecodeArgs : tread_paged_attn_args {
   int G;
   float scale_log2;
   unsigned* err;
-  int4* desc;   // [kMaxCtas] {parts of the item that starts in this CTA and ends in another, b, g, slot}
+  // {parts, state of the first, b, g} of the items that the join has to look at: by item (b Hkv + g) where
+  // there are no more of them than CTAs, else by the CTA in which an item starts that ends in another
+  int4* desc;  // [kMaxCtas]
   float2* ml;   // [kMaxCtas][2][G] {maximum, sum} of the partial states
   float* part;  // [kMaxCtas][2][G][D]
 };
+
+__host__ __device__ __forceinline__ bool by_items(const DecodeArgs& a, int ctas) {
+  return (long long)a.B * a.Hkv <= ctas;
+}
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) {
   return static_cast<unsigned>(__cvta_generic_to_shared(p));
@@ -177,7 +184,7 @@ struct MmaState {
       }
     }
     const bool live0 = (live >> (lane >> 2)) & 1, live1 = (live >> ((lane >> 2) + 8)) & 1;
-    unsigned p[NT][2];
+    unsigned p[NT][2], rest[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[4];
@@ -208,6 +215,10 @@ struct MmaState {
       l[nt][1] += x[1] + x[3];
       p[nt][0] = transpose8x8(pack2<T>(x[0], x[1]));
       p[nt][1] = transpose8x8(pack2<T>(x[2], x[3]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] -= Num<T>::to_f(Num<T>::from_f(x[i]));
+      rest[nt][0] = transpose8x8(pack2<T>(x[0], x[1]));
+      rest[nt][1] = transpose8x8(pack2<T>(x[2], x[3]));
     }
     {
       const int row = (lane & 7) + ((lane >> 4) << 3);
@@ -217,7 +228,10 @@ struct MmaState {
         unsigned f[4];
         ldmatrix_x4_trans(f, base + (((2 * mt + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][mt], f, p[nt]);
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<T>(o[nt][mt], f, p[nt]);
+          mma16816<T>(o[nt][mt], f, rest[nt]);
+        }
       }
     }
   }
@@ -376,6 +390,11 @@ __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
 }
 __device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kUnit; }
 
+// x / y, by the short division where it will do
+__device__ __forceinline__ long long quotient(long long x, unsigned y) {
+  return (x >> 32) == 0 ? (long long)((unsigned)x / y) : x / y;
+}
+
 // A place on the line of units: unit j of item (b, g), the item having n units of len tokens.
 struct Place {
   int b, g, j, n, len;
@@ -446,25 +465,27 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
     total += s_scan[w], total_items += s_items[w];
   }
   const long long line = (total + (long long)kItemCost * total_items) * a.Hkv;
-  long long share = (line + gridDim.x - 1) / gridDim.x;
+  long long share = quotient(line + gridDim.x - 1, gridDim.x);
   if (share < kMinShare) share = kMinShare;
   // the share's ends on the line of units alone, and the place of its first unit
   const long long c0 = min(line, blockIdx.x * share), c1 = min(line, c0 + share);
   const long long run0 = (before + (long long)kItemCost * before_items) * a.Hkv;
   const long long run1 = run0 + (units + (long long)kItemCost * items) * a.Hkv;
-  if (threadIdx.x == 0) s_ends[0] = s_ends[1] = total * a.Hkv;  // of a cut at the line's end
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    __syncthreads();
     const long long cut = i == 0 ? c0 : c1;
-    if (cut < run0 || cut >= run1) continue;
+    if (cut >= line) {
+      if (threadIdx.x == 0) s_ends[i] = total * a.Hkv;
+      continue;
+    }
+    if (cut < run0 || cut >= run1) continue;  // in another thread's run
     long long at = run0, at_units = before * a.Hkv;
     for (int b = b0;; ++b) {
       const int len = length_of(a, b), n = units_of(len);
       const long long here = len > 0 ? (long long)(n + kItemCost) * a.Hkv : 0;
       if (cut < at + here) {
-        const long long in = cut - at;
-        const int g = (int)(in / (n + kItemCost)), j = max(0, (int)(in % (n + kItemCost)) - kItemCost);
+        const int g = (int)quotient(cut - at, n + kItemCost);
+        const int j = max(0, (int)(cut - at - (long long)g * (n + kItemCost)) - kItemCost);
         s_ends[i] = at_units + (long long)g * n + j;
         if (i == 0) s_place = Place{b, g, j, n, len};
         break;
@@ -474,28 +495,38 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
     }
   }
   // sequences without a key: zeros
+  const bool by_item = by_items(a, gridDim.x);
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-    if (length_of(a, b) == 0)
+    if (length_of(a, b) == 0) {
       for (int i = threadIdx.x; i < a.Hq * D; i += kThreads)
         static_cast<T*>(a.out)[(long long)b * a.Hq * D + i] = Num<T>::from_f(0.f);
+      if (by_item)
+        for (int g = threadIdx.x; g < a.Hkv; g += kThreads) a.desc[b * a.Hkv + g] = make_int4(0, 0, 0, 0);
+    }
   __syncthreads();
   const long long u0 = s_ends[0], u1 = s_ends[1];
   if (u0 >= u1) {
-    if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0 && !by_item) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
 
-  // the warp's own walk along the share, kStages - 1 units ahead of what it computes
-  Place load = s_place;
+  typename StateOf<T, D, GP>::type st;
+  st.start(a, s_place.b, s_place.g, extra, warp, lane);  // the first item's queries are on their way
+
+  // the warp's own walk along the share, kStages - 1 units ahead of what it computes; the pages' numbers are
+  // read a unit further ahead
+  Place load = s_place, next = load;
   load.j += warp;
   load.settle(a);
+  next = load;
+  next.j += W;
+  next.settle(a);
   long long load_at = u0 + warp;
-  auto page_of = [&]() -> int {  // of the unit's first key, or of the lane's key
-    const unsigned t = load.j * kUnit + (WHOLE ? 0 : lane & 15);
-    return load_at < u1 && t < (unsigned)load.len ? __ldg(a.table + load.b * a.table_ld + t / (unsigned)a.page_size)
-                                                  : -1;
+  auto page_of = [&](const Place& p, long long at) -> int {  // of the unit's first key, or of the lane's key
+    const unsigned t = p.j * kUnit + (WHOLE ? 0 : lane & 15);
+    return at < u1 && t < (unsigned)p.len ? __ldg(a.table + p.b * a.table_ld + t / (unsigned)a.page_size) : -1;
   };
-  int id = page_of();
+  int id = page_of(load, load_at), next_id = page_of(next, load_at + W);
   auto fetch = [&](int stage) {
     if (load_at < u1) {
       constexpr int kChunks = S::kRow / 16, kIter = kUnit * kChunks / 32;
@@ -529,9 +560,11 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
         cp_async16(to + kUnit * S::kRow, vp + (read ? from : 0), read);
       }
       load_at += W;
-      load.j += W;
-      load.settle(a);
-      id = page_of();
+      load = next;
+      id = next_id;
+      next.j += W;
+      next.settle(a);
+      next_id = page_of(next, load_at + W);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -542,10 +575,9 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
   long long pos = u0;
   int step = 0;  // the warp's units so far, modulo the ring
   int4 open = make_int4(0, 0, 0, 0);
-  typename StateOf<T, D, GP>::type st;
   while (pos < u1) {
     const int seg = (int)min((long long)(at.n - at.j), u1 - pos);
-    st.start(a, at.b, at.g, extra, warp, lane);
+    if (pos != u0) st.start(a, at.b, at.g, extra, warp, lane);
     const int skip = (int)((pos - u0) % W);
     for (int i = warp >= skip ? warp - skip : warp - skip + W; i < seg; i += W) {
       cp_async_wait<kStages - 2>();
@@ -562,43 +594,52 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
     const bool whole = seg == at.n;
     const int slot = pos == u0 ? 0 : 1;
     const long long p = (long long)blockIdx.x * 2 + slot;
-    for (int i = threadIdx.x; i < a.G * (D / 2); i += kThreads) {
-      const int h = i / (D / 2), d = i % (D / 2) * 2;
-      float top = -INFINITY;
+    for (int i = threadIdx.x; i < a.G * (D / 8); i += kThreads) {  // eight elements of a head
+      const int h = i / (D / 8), d = i % (D / 8) * 8;
+      float top = -INFINITY, sum = 0.f, x[8] = {};
 #pragma unroll
       for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][h].x);
-      float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         const float f = weight(s_ml[w][h].x, top);
-        const float2 o = *reinterpret_cast<const float2*>(s_o + w * GP * D + place_of<D>(h, d));
+        const float4* o = reinterpret_cast<const float4*>(s_o + w * GP * D + place_of<D>(h, d));
+        const float4 y = o[0], z = o[1];
         sum += f * s_ml[w][h].y;
-        x += f * o.x;
-        y += f * o.y;
+        x[0] += f * y.x, x[1] += f * y.y, x[2] += f * y.z, x[3] += f * y.w;
+        x[4] += f * z.x, x[5] += f * z.y, x[6] += f * z.z, x[7] += f * z.w;
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         T* to = static_cast<T*>(a.out) + ((long long)at.b * a.Hq + at.g * a.G + h) * D + d;
-        to[0] = Num<T>::from_f(x * inv);
-        to[1] = Num<T>::from_f(y * inv);
+        constexpr int E = 16 / sizeof(T);
+#pragma unroll
+        for (int k = 0; k < 8; k += E) {
+          Vec16<T> v;
+#pragma unroll
+          for (int e = 0; e < E; ++e) v.e[e] = Num<T>::from_f(x[k + e] * inv);
+          *reinterpret_cast<int4*>(to + k) = v.raw;
+        }
       } else {
-        *reinterpret_cast<float2*>(a.part + (p * a.G + h) * D + d) = make_float2(x, y);
+        float4* to = reinterpret_cast<float4*>(a.part + (p * a.G + h) * D + d);
+        to[0] = make_float4(x[0], x[1], x[2], x[3]);
+        to[1] = make_float4(x[4], x[5], x[6], x[7]);
         if (d == 0) a.ml[p * a.G + h] = make_float2(top, sum);
       }
     }
     if (!whole && at.j == 0)  // starts here, ends in the CTA of its last unit
-      open = make_int4((int)((c1 + at.n - seg - 1) / share - blockIdx.x + 1), at.b, at.g, slot);
+      open = make_int4((int)((c1 + at.n - seg - 1) / share - blockIdx.x + 1), (int)p, at.b, at.g);
+    if (by_item && at.j == 0 && threadIdx.x == 0)
+      a.desc[at.b * a.Hkv + at.g] = whole ? make_int4(0, 0, 0, 0) : open;
     pos += seg;
     at.j += seg;
     if (pos < u1) at.settle(a);
     __syncthreads();
   }
   cp_async_wait<0>();
-  if (threadIdx.x == 0) a.desc[blockIdx.x] = open;
+  if (threadIdx.x == 0 && !by_item) a.desc[blockIdx.x] = open;
 }
 
-// Items whose keys several CTAs share: CTA (c, h) joins head h of the item that starts in share c and
-// ends in another. All parts' maxima and sums are read at once and turned into weights; the warps then take
+// Items whose keys several CTAs share: CTA (i, h) joins head h of the item that desc[i] names. All parts' maxima and sums are read at once and turned into weights; the warps then take
 // the accumulators in turn, kAhead loads in flight each.
 constexpr int kJoinWarps = 8;
 
@@ -610,7 +651,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
   const int4 open = a.desc[blockIdx.x];
   if (open.x == 0) return;
   const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto state = [&](int i) { return ((blockIdx.x + i) * 2LL + (i == 0 ? open.w : 0)) * a.G + h; };
+  // the first part is in either of its CTA's slots, the others in their CTAs' first
+  auto state = [&](int i) { return (long long)(i == 0 ? open.y : (open.y / 2 + i) * 2) * a.G + h; };
   float o[kPer] = {};
   float2 ml[(kMaxCtas + kThreads - 1) / kThreads];
   float top = -INFINITY, sum = 0.f;
@@ -666,7 +708,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) all += s_l[w];
   const float inv = all == 0.f ? 0.f : 1.f / all;
-  T* to = static_cast<T*>(a.out) + ((long long)open.y * a.Hq + open.z * a.G + h) * D;
+  T* to = static_cast<T*>(a.out) + ((long long)open.z * a.Hq + open.w * a.G + h) * D;
   for (int d = threadIdx.x; d < D; d += kThreads) {
     float x = 0.f;
 #pragma unroll
@@ -688,7 +730,7 @@ int launch(const DecodeArgs& a, int sms, cudaStream_t st) {
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, a.G);
+  cfg.gridDim = dim3(by_items(a, ctas) ? a.B * a.Hkv : ctas, a.G);
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cfg.attrs = &attr;
