@@ -43,6 +43,7 @@ def _attn_call(**over):
     (dict(page=0), "page geometry"), (dict(hs=16), "page geometry"), (dict(table=None), "page table"),
     (dict(t_ld=2), "page table"), (dict(q=264), "16-byte"), (dict(kp=264), "16-byte"), (dict(out=264), "16-byte"),
     (dict(q_ld=516), "16-byte"), (dict(ps=2 * 16 * 128 + 4), "16-byte"), (dict(P=2 ** 28, t_ld=2 ** 28), "2^31"),
+    (dict(P=2 ** 26, t_ld=2 ** 26, B=9), "2^34"),
     (dict(ws=None), "workspace"), (dict(ws=264), "workspace"), (dict(ws_bytes=100), "workspace"),
 ])
 def test_paged_attn_rejects_bad_arguments(over, needle):

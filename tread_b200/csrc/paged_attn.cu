@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kUnit = 16;      // keys of one unit
 constexpr int kMaxCtas = 384;  // shares at most
-constexpr int kItemCost = 4;   // units that an item's fixed cost amounts to
+constexpr int kItemCost = 8;   // units that an item's fixed cost amounts to
 constexpr int kMinShare = 4;   // a unit for every warp: more parts cost more to join
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // the running maximum may lag by 2^8: weights stay far inside fp16's range
@@ -57,6 +57,7 @@ __device__ __forceinline__ unsigned smem_addr(const void* p) {
   return static_cast<unsigned>(__cvta_generic_to_shared(p));
 }
 
+// 16 bytes, zeros where `read` is false
 __device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool read) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
 }
@@ -390,11 +391,6 @@ __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
 }
 __device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kUnit; }
 
-// x / y, by the short division where it will do
-__device__ __forceinline__ long long quotient(long long x, unsigned y) {
-  return (x >> 32) == 0 ? (long long)((unsigned)x / y) : x / y;
-}
-
 // A place on the line of units: unit j of item (b, g), the item having n units of len tokens.
 struct Place {
   int b, g, j, n, len;
@@ -421,23 +417,23 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
     paged_attn_kernel(const __grid_constant__ DecodeArgs a) {
   using S = Shape<T, D, GP>;
   constexpr int W = S::kWarps, kThreads = W * 32, kStages = S::kStages;
+  static_assert((W & (W - 1)) == 0, "the warps' turns");
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ unsigned s_live[W][kStages];
   __shared__ float2 s_ml[W][GP];
-  __shared__ long long s_scan[W], s_ends[2];
-  __shared__ int s_items[W];
+  __shared__ int2 s_scan[W];
+  __shared__ int s_ends[2];
   __shared__ Place s_place;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* s_o = reinterpret_cast<float*>(smem + kStages * W * S::kUnitBytes);
   void* extra = smem + kStages * W * S::kUnitBytes + S::kJoin;
   const unsigned ring = smem_addr(smem) + warp * (kStages * S::kUnitBytes);
 
-  // the line: every thread adds up a run of sequences, a scan places the runs. Units and items are summed side
-  // by side (a sequence has under 2^27 units; 2^32 sequences there are not).
+  // the line: every thread adds up a run of sequences, a scan places the runs. An item's weight is its units and
+  // kItemCost; units and weights are summed side by side (the caller has made sure that they fit).
   const int run = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(a.B, (int)threadIdx.x * run), b1 = min(a.B, b0 + run);
-  long long units = 0;
-  int items = 0;
+  int units = 0, items = 0;
   for (int b = b0; b < b1; ++b) {
     const int len = length_of(a, b);
     units += units_of(len);
@@ -447,51 +443,44 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
       if (n != 0 && a.err) atomicOr(a.err, 2u);
     }
   }
-  long long upto = units;
-  int upto_items = items;
+  int upto = units, upto_items = items;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, upto, off);
-    const int y = __shfl_up_sync(0xffffffffu, upto_items, off);
+    const int x = __shfl_up_sync(0xffffffffu, upto, off), y = __shfl_up_sync(0xffffffffu, upto_items, off);
     if (lane >= off) upto += x, upto_items += y;
   }
-  if (lane == 31) s_scan[warp] = upto, s_items[warp] = upto_items;
+  if (lane == 31) s_scan[warp] = make_int2(upto, upto_items);
   __syncthreads();
-  long long before = upto - units, total = 0;
-  int before_items = upto_items - items, total_items = 0;
+  int before = upto - units, total = 0, before_items = upto_items - items, total_items = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    if (w < warp) before += s_scan[w], before_items += s_items[w];
-    total += s_scan[w], total_items += s_items[w];
+    if (w < warp) before += s_scan[w].x, before_items += s_scan[w].y;
+    total += s_scan[w].x, total_items += s_scan[w].y;
   }
-  const long long line = (total + (long long)kItemCost * total_items) * a.Hkv;
-  long long share = quotient(line + gridDim.x - 1, gridDim.x);
-  if (share < kMinShare) share = kMinShare;
+  const int line = (total + kItemCost * total_items) * a.Hkv;
+  const int share = max(kMinShare, (line + (int)gridDim.x - 1) / (int)gridDim.x);
   // the share's ends on the line of units alone, and the place of its first unit
-  const long long c0 = min(line, blockIdx.x * share), c1 = min(line, c0 + share);
-  const long long run0 = (before + (long long)kItemCost * before_items) * a.Hkv;
-  const long long run1 = run0 + (units + (long long)kItemCost * items) * a.Hkv;
-#pragma unroll
+  const int c0 = min(line, (int)blockIdx.x * share), c1 = min(line, c0 + share);
+  const int run0 = (before + kItemCost * before_items) * a.Hkv, run1 = run0 + (units + kItemCost * items) * a.Hkv;
+#pragma unroll 1
   for (int i = 0; i < 2; ++i) {
-    const long long cut = i == 0 ? c0 : c1;
+    const int cut = i == 0 ? c0 : c1;
     if (cut >= line) {
       if (threadIdx.x == 0) s_ends[i] = total * a.Hkv;
       continue;
     }
     if (cut < run0 || cut >= run1) continue;  // in another thread's run
-    long long at = run0, at_units = before * a.Hkv;
+    int at = run0, at_units = before * a.Hkv;
     for (int b = b0;; ++b) {
-      const int len = length_of(a, b), n = units_of(len);
-      const long long here = len > 0 ? (long long)(n + kItemCost) * a.Hkv : 0;
-      if (cut < at + here) {
-        const int g = (int)quotient(cut - at, n + kItemCost);
-        const int j = max(0, (int)(cut - at - (long long)g * (n + kItemCost)) - kItemCost);
-        s_ends[i] = at_units + (long long)g * n + j;
+      const int len = length_of(a, b), n = units_of(len), weight = len > 0 ? n + kItemCost : 0;
+      if (cut < at + weight * a.Hkv) {
+        const int g = (cut - at) / weight, j = max(0, cut - at - g * weight - kItemCost);
+        s_ends[i] = at_units + g * n + j;
         if (i == 0) s_place = Place{b, g, j, n, len};
         break;
       }
-      at += here;
-      at_units += (long long)n * a.Hkv;
+      at += weight * a.Hkv;
+      at_units += n * a.Hkv;
     }
   }
   // sequences without a key: zeros
@@ -504,7 +493,7 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
         for (int g = threadIdx.x; g < a.Hkv; g += kThreads) a.desc[b * a.Hkv + g] = make_int4(0, 0, 0, 0);
     }
   __syncthreads();
-  const long long u0 = s_ends[0], u1 = s_ends[1];
+  const int u0 = s_ends[0], u1 = s_ends[1];
   if (u0 >= u1) {
     if (threadIdx.x == 0 && !by_item) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
@@ -513,7 +502,7 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
   typename StateOf<T, D, GP>::type st;
   st.start(a, s_place.b, s_place.g, extra, warp, lane);  // the first item's queries are on their way
 
-  // the warp's own walk along the share, kStages - 1 units ahead of what it computes; the pages' numbers are
+  // the warp's own walk along the share, kStages units ahead of what it computes; the pages' numbers are
   // read a unit further ahead
   Place load = s_place, next = load;
   load.j += warp;
@@ -521,8 +510,8 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
   next = load;
   next.j += W;
   next.settle(a);
-  long long load_at = u0 + warp;
-  auto page_of = [&](const Place& p, long long at) -> int {  // of the unit's first key, or of the lane's key
+  int load_at = u0 + warp;
+  auto page_of = [&](const Place& p, int at) -> int {  // of the unit's first key, or of the lane's key
     const unsigned t = p.j * kUnit + (WHOLE ? 0 : lane & 15);
     return at < u1 && t < (unsigned)p.len ? __ldg(a.table + p.b * a.table_ld + t / (unsigned)a.page_size) : -1;
   };
@@ -536,29 +525,39 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
       const unsigned slot = t - t / (unsigned)a.page_size * a.page_size;
       const long long off = known ? id * a.page_stride + load.g * a.head_stride + (long long)slot * D : 0;
       const int rows = min(kUnit, load.len - (int)t0);
-      unsigned live = (1u << rows) - 1;
-      if (WHOLE) {
-        if (!known) live = 0;
-      } else {
-        live &= __ballot_sync(0xffffffffu, known);  // lanes 16..31 repeat lanes 0..15
-      }
-      if (live != (1u << rows) - 1 && lane == 0 && a.err) atomicOr(a.err, 2u);
-      if (lane == 0) s_live[warp][stage] = live;
       const char* kp = static_cast<const char*>(a.k_pages);
       const char* vp = static_cast<const char*>(a.v_pages);
+      unsigned live = (1u << rows) - 1;
+      if (WHOLE && known && rows == kUnit) {  // the common unit: 16 rows that follow each other
+        kp += off * (int)sizeof(T) + lane * 16;
+        vp += off * (int)sizeof(T) + lane * 16;
+        constexpr int kRows = kChunks < 32 ? 32 / kChunks : 1;  // rows of one step of 512 bytes
+        const unsigned to = dst + (kChunks < 32 ? lane / kChunks * S::kRow + (((lane % kChunks) ^ (lane / kChunks)) << 4) : lane << 4);
 #pragma unroll
-      for (int it = 0; it < kIter; ++it) {
-        const int row = (it * 32 + lane) / kChunks, c = (it * 32 + lane) % kChunks;
-        long long from;
-        if constexpr (WHOLE)
-          from = (off + (long long)row * D) * (int)sizeof(T) + c * 16;
-        else
-          from = __shfl_sync(0xffffffffu, off, row) * (int)sizeof(T) + c * 16;
-        const bool read = (live >> row) & 1;
-        const unsigned to = dst + row * S::kRow + ((c ^ (row & 7)) << 4);
-        cp_async16(to, kp + (read ? from : 0), read);  // rows that are not read are zero
-        cp_async16(to + kUnit * S::kRow, vp + (read ? from : 0), read);
+        for (int it = 0; it < kIter; ++it) {
+          const int row = kChunks <= 32 ? it * kRows : it * 32 / kChunks;  // the step's first row
+          const unsigned at = (to ^ ((row & 7) << 4)) + (kChunks <= 32 ? row * S::kRow : it * 512);
+          cp_async16(at, kp + it * 512, true);
+          cp_async16(at + kUnit * S::kRow, vp + it * 512, true);
+        }
+      } else {
+        if (WHOLE) {
+          if (!known) live = 0;
+        } else {
+          live &= __ballot_sync(0xffffffffu, known);  // lanes 16..31 repeat lanes 0..15
+        }
+        if (live != (1u << rows) - 1 && lane == 0 && a.err) atomicOr(a.err, 2u);
+#pragma unroll 1
+        for (int it = 0; it < kIter; ++it) {
+          const int row = (it * 32 + lane) / kChunks, c = (it * 32 + lane) % kChunks;
+          const long long from = ((WHOLE ? off + row * D : __shfl_sync(0xffffffffu, off, row))) * (int)sizeof(T) + c * 16;
+          const bool read = (live >> row) & 1;
+          const unsigned to = dst + row * S::kRow + ((c ^ (row & 7)) << 4);
+          cp_async16(to, kp + (read ? from : 0), read);  // rows that are not read are zero
+          cp_async16(to + kUnit * S::kRow, vp + (read ? from : 0), read);
+        }
       }
+      if (lane == 0) s_live[warp][stage] = live;
       load_at += W;
       load = next;
       id = next_id;
@@ -568,32 +567,36 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(i);
-
   Place at = s_place;
-  long long pos = u0;
-  int step = 0;  // the warp's units so far, modulo the ring
+  int pos = u0;
+  int step = 0;              // the warp's units so far, modulo the ring
+  int slot = 0, owed = kStages;  // the ring's next slot to fill, and how many are free
   int4 open = make_int4(0, 0, 0, 0);
   while (pos < u1) {
-    const int seg = (int)min((long long)(at.n - at.j), u1 - pos);
+    const int seg = min(at.n - at.j, u1 - pos);
     if (pos != u0) st.start(a, at.b, at.g, extra, warp, lane);
-    const int skip = (int)((pos - u0) % W);
-    for (int i = warp >= skip ? warp - skip : warp - skip + W; i < seg; i += W) {
-      cp_async_wait<kStages - 2>();
+    // one more turn than there are units, for the slots that the last one (or nothing yet) has left free: the
+    // code of a fetch is in one place, since a short share's time is mostly that of reading instructions
+    for (int i = (warp - (pos - u0)) & (W - 1);; i += W) {
+#pragma unroll 1
+      for (; owed > 0; --owed) {
+        fetch(slot);
+        slot = slot + 1 == kStages ? 0 : slot + 1;
+      }
+      if (i >= seg) break;
+      cp_async_wait<kStages - 1>();
       __syncwarp();
       const unsigned stage = ring + step * S::kUnitBytes;
-      const unsigned live = s_live[warp][step];
-      fetch(step == 0 ? kStages - 1 : step - 1);  // into the place of the unit before, which every lane has read
-      st.unit(a, stage, stage + kUnit * S::kRow, live, extra, warp, lane);
+      st.unit(a, stage, stage + kUnit * S::kRow, s_live[warp][step], extra, warp, lane);
       step = step + 1 == kStages ? 0 : step + 1;
+      owed = 1;
+      __syncwarp();  // every lane has read the unit before its place is filled again
     }
     // the item's end, or the share's: join the warps
     st.leave(s_o + warp * GP * D, s_ml[warp], lane);
     __syncthreads();
     const bool whole = seg == at.n;
-    const int slot = pos == u0 ? 0 : 1;
-    const long long p = (long long)blockIdx.x * 2 + slot;
+    const long long p = (long long)blockIdx.x * 2 + (pos == u0 ? 0 : 1);
     for (int i = threadIdx.x; i < a.G * (D / 8); i += kThreads) {  // eight elements of a head
       const int h = i / (D / 8), d = i % (D / 8) * 8;
       float top = -INFINITY, sum = 0.f, x[8] = {};
@@ -627,7 +630,7 @@ __global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
       }
     }
     if (!whole && at.j == 0)  // starts here, ends in the CTA of its last unit
-      open = make_int4((int)((c1 + at.n - seg - 1) / share - blockIdx.x + 1), (int)p, at.b, at.g);
+      open = make_int4((c1 + at.n - seg - 1) / share - (int)blockIdx.x + 1, (int)p, at.b, at.g);
     if (by_item && at.j == 0 && threadIdx.x == 0)
       a.desc[at.b * a.Hkv + at.g] = whole ? make_int4(0, 0, 0, 0) : open;
     pos += seg;
@@ -782,6 +785,8 @@ extern "C" int tread_paged_attn(const tread_paged_attn_args* args, tread_stream_
                   "paged_attn: bad page table");
   TREAD_CHECK_ARG((int64_t)a.max_pages * a.page_size <= INT32_MAX - kUnit,
                   "paged_attn: a sequence of 2^31 tokens or more");
+  TREAD_CHECK_ARG(((int64_t)a.max_pages * a.page_size / kUnit + 1 + kItemCost) * a.Hkv <= (1 << 30) / a.B,
+                  "paged_attn: a table of more than 2^34 tokens, counted by KV head");
   TREAD_CHECK_ARG(aligned16(a.q) && aligned16(a.k_pages) && aligned16(a.v_pages) && aligned16(a.out) &&
                       ((a.q_ld | a.page_stride | a.head_stride) * es) % 16 == 0,
                   "paged_attn: q, out and pages must lie on 16-byte boundaries");
