@@ -502,14 +502,22 @@ def _index(t, n, dtype, name):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of length {n}")
 
 
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 def _elsewhere(index, stream):
-    """The context in which a call on tensors of CUDA device `index` has to run, or None where it is the
-    current one: launches and allocations go to the current device and stream."""
-    if stream is not None:
-        if stream.device.index != index:
-            raise ValueError(f"the stream is on {stream.device}, the call's tensors on cuda:{index}")
-        return torch.cuda.stream(stream)
-    return None if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+    """The context of a call on tensors of CUDA device `index`: launches and allocations go to the current
+    device and stream."""
+    if stream is None:
+        return torch.cuda.device(index)
+    if stream.device.index != index:
+        raise ValueError(f"the stream is on {stream.device}, the call's tensors on cuda:{index}")
+    return torch.cuda.stream(stream)
+
+
+def _on(t, index, name):
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{index}")
 
 
 def _launch(name, index, args):
@@ -541,51 +549,62 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
     Returns the rotated queries [R, Hq, D] (q_out, which may be q itself), or None without q."""
     (N, Hkv, page_size, D), sp, sh = _pages(k_pages, v_pages)
     index = k_pages.get_device()
-    other = _elsewhere(index, stream)
-    if other is not None:
-        with other:
+    if stream is not None or _current_device() != index:
+        with _elsewhere(index, stream):
             return paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out, err)
     if not (k.get_device() == v.get_device() == v_pages.get_device() == table.get_device() == pos.get_device() == index):
         C.same_device(k_pages, k=k, v=v, v_pages=v_pages, table=table, pos=pos)
     dtype, shape = k.dtype, k.shape
-    k_stride, v_stride = k.stride(), v.stride()
-    if len(shape) != 3 or shape[1] != Hkv or shape[2] != D or v.shape != shape or k_stride[2] != 1 or v_stride[2] != 1:
+    k_ld, k_sh, k_last = k.stride() if len(shape) == 3 else (0, 0, 0)
+    if k_last != 1 or shape[1] != Hkv or shape[2] != D or v.shape != shape or v.stride(2) != 1:
         raise ValueError(f"k and v must be [R, {Hkv}, {D}] with unit last stride")
     if not (dtype == v.dtype == k_pages.dtype):
         raise TypeError("k, v and the pages must share a dtype")
     R = shape[0]
+    v_ld, v_sh, _ = v.stride()
     ld, S, width = _table(table)
-    _index(pos, R, torch.int64, "pos")
+    at = (R,)
+    if pos.shape != at or pos.dtype != torch.int64 or not pos.is_contiguous():
+        _index(pos, R, torch.int64, "pos")
+    seq_ptr = rope_ptr = inv_ptr = err_ptr = q_ptr = out_ptr = Hq = q_ld = q_sh = 0
     if seq is not None:
         _index(seq, R, torch.int32, "seq")
+        _on(seq, index, "seq")
+        seq_ptr = seq.data_ptr()
     elif R > S:
         raise ValueError(f"{R} rows without seq, but a table of {S} sequences")
     if rope_pos is not None:
         _index(rope_pos, R, torch.int64, "rope_pos")
+        _on(rope_pos, index, "rope_pos")
+        rope_ptr = rope_pos.data_ptr()
     if inv_freq is not None:
         _index(inv_freq, D // 2, torch.float32, "inv_freq")
-    Hq = q_ld = q_sh = 0
-    if q is None:
-        if q_out is not None:
-            raise ValueError("q_out without q")
-    else:
-        shape, q_stride = q.shape, q.stride()
-        if len(shape) != 3 or shape[0] != R or shape[2] != D or q_stride[2] != 1 or q.dtype != dtype:
+        _on(inv_freq, index, "inv_freq")
+        inv_ptr = inv_freq.data_ptr()
+    if err is not None:
+        _on(err, index, "err")
+        err_ptr = err.data_ptr()
+    if q is not None:
+        shape = q.shape
+        q_ld, q_sh, q_last = q.stride() if len(shape) == 3 else (0, 0, 0)
+        if q_last != 1 or shape[0] != R or shape[2] != D or q.dtype != dtype:
             raise ValueError(f"q must be [{R}, Hq, {D}] of k's dtype with unit last stride")
         if inv_freq is None:
             raise ValueError("q without inv_freq: nothing rotates it")
-        Hq, q_ld, q_sh = shape[1], q_stride[0], q_stride[1]
+        _on(q, index, "q")
         if q_out is None:
             q_out = q.new_empty(shape)
         elif q_out.shape != shape or q_out.dtype != dtype or not q_out.is_contiguous():
             raise ValueError(f"q_out must be a contiguous {tuple(shape)} tensor of q's dtype")
-    for t in (seq, rope_pos, inv_freq, q, q_out, err):
-        if t is not None and t.get_device() != index:
-            C.same_device(k_pages, seq=seq, inv_freq=inv_freq, rope_pos=rope_pos, q=q, q_out=q_out, err=err)
+        else:
+            _on(q_out, index, "q_out")
+        Hq, q_ptr, out_ptr = shape[1], q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
     _launch("tread_paged_append", index, C.PAGED_APPEND.pack(
-        k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
-        _ptr(seq), pos.data_ptr(), _ptr(rope_pos), _ptr(inv_freq), _ptr(err), k_stride[0], k_stride[1], v_stride[0],
-        v_stride[1], q_ld, q_sh, sp, sh, N, ld, page_size, S, width, R, Hq, Hkv, D, C.dtype_code(dtype), attn_scaling))
+        k.data_ptr(), v.data_ptr(), q_ptr, out_ptr, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), seq_ptr,
+        pos.data_ptr(), rope_ptr, inv_ptr, err_ptr, k_ld, k_sh, v_ld, v_sh, q_ld, q_sh, sp, sh, N, ld, page_size, S, width,
+        R, Hq, Hkv, D, C.dtype_code(dtype), attn_scaling))
     return q_out
 
 
@@ -598,13 +617,11 @@ def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=No
     1, and so does a page id outside the pool, whose keys count as masked. Returns out [B, Hq, D]."""
     (N, Hkv, page_size, D), sp, sh = _pages(k_pages, v_pages)
     index = k_pages.get_device()
-    other = _elsewhere(index, stream)
-    if other is not None:
-        with other:
+    if stream is not None or _current_device() != index:
+        with _elsewhere(index, stream):
             return paged_attn(q, k_pages, v_pages, table, lens, out, sm_scale, err)
-    if not (q.get_device() == v_pages.get_device() == table.get_device() == lens.get_device() == index) or (
-            out is not None or err is not None):
-        C.same_device(k_pages, q=q, v_pages=v_pages, table=table, lens=lens, out=out, err=err)
+    if not (q.get_device() == v_pages.get_device() == table.get_device() == lens.get_device() == index):
+        C.same_device(k_pages, q=q, v_pages=v_pages, table=table, lens=lens)
     shape, stride, dtype = q.shape, q.stride(), q.dtype
     if len(shape) != 3 or shape[2] != D or stride[2] != 1 or (shape[1] > 1 and stride[1] != D) or dtype != k_pages.dtype:
         raise ValueError(f"q must be [B, Hq, {D}] of the pages' dtype with contiguous rows")
@@ -617,11 +634,17 @@ def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=No
         out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(shape)} tensor of q's dtype")
+    else:
+        _on(out, index, "out")
+    err_ptr = 0
+    if err is not None:
+        _on(err, index, "err")
+        err_ptr = err.data_ptr()
     # one workspace a call, from the allocator: calls of several streams, threads and graphs share none
     nbytes = C.lib().tread_paged_attn_workspace_bytes(Hq, Hkv, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     _launch("tread_paged_attn", index, C.PAGED_ATTN.pack(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), _ptr(err),
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), err_ptr,
         ws.data_ptr(), stride[0], sp, sh, N, ld, nbytes, page_size, width, B, Hq, Hkv, D, C.dtype_code(dtype),
         D ** -0.5 if sm_scale is None else sm_scale))
     return out
@@ -662,9 +685,8 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
     Returns out: fp32 [B, V] by default; a given one may be of any supported dtype, or logits itself."""
     C.require_cuda(logits, "logits")
     index = logits.get_device()
-    other = _elsewhere(index, stream)
-    if other is not None:
-        with other:
+    if stream is not None or _current_device() != index:
+        with _elsewhere(index, stream):
             return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
                                  allowed, out)
     shape, stride = logits.shape, logits.stride()
