@@ -1,7 +1,14 @@
 """Host-side argument checks of the decode-step entry points (no GPU: nothing is launched)."""
+import struct
+
 import pytest
 
 from tread_b200 import _capi as C
+
+# the argument structs' fields in order, natively aligned
+PAGED_APPEND = struct.Struct("@12P10q8if0q")
+PAGED_ATTN = struct.Struct("@8P6q7if")
+ADJUST_LOGITS = struct.Struct("@11P6q6i3f0q")
 
 
 def _append_call(**over):
@@ -9,7 +16,7 @@ def _append_call(**over):
              vp=256, ps=2 * 16 * 128, hs=16 * 128, N=8, page=16, table=256, t_ld=4, S=4, P=4, seq=None, pos=256,
              rpos=None, R=3, Hq=4, Hkv=2, D=128, inv=256, scale=1.0, err=None, dtype=C.TREAD_BF16)
     a.update(over)
-    return C.lib().tread_paged_append(C.PAGED_APPEND.pack(*(a[n] or 0 for n in (
+    return C.lib().tread_paged_append(PAGED_APPEND.pack(*(a[n] or 0 for n in (
         "k v q q_out kp vp table seq pos rpos inv err k_ld k_sh v_ld v_sh q_ld q_sh ps hs N t_ld page S P R Hq Hkv D dtype "
         "scale").split())), None)
 
@@ -33,7 +40,7 @@ def _attn_call(**over):
     a.update(over)
     n = C.lib().tread_paged_attn_workspace_bytes(4, 2, 128) if a["ws_bytes"] is None else a["ws_bytes"]
     a["ws_bytes"] = n
-    return C.lib().tread_paged_attn(C.PAGED_ATTN.pack(*(a[k] or 0 for k in (
+    return C.lib().tread_paged_attn(PAGED_ATTN.pack(*(a[k] or 0 for k in (
         "q kp vp out table lens err ws q_ld ps hs N t_ld ws_bytes page P B Hq Hkv D dtype scale").split())), None)
 
 
@@ -56,7 +63,7 @@ def _logits_call(**over):
              rep_all=1.2, pres=None, pres_all=0.0, freq=None, freq_all=0.0, ids=256, ids_ld=2, bias=256, bias_ld=2,
              nb=2, allowed=256, al_ld=4, dtype=C.TREAD_BF16, odt=C.TREAD_F32)
     a.update(over)
-    return C.lib().tread_adjust_logits(C.ADJUST_LOGITS.pack(*(a[k] or 0 for k in (
+    return C.lib().tread_adjust_logits(ADJUST_LOGITS.pack(*(a[k] or 0 for k in (
         "x out tok lens plens rep pres freq ids bias allowed ld ld_out tok_ld ids_ld bias_ld al_ld B V H nb dtype odt "
         "rep_all pres_all freq_all").split())), None)
 
@@ -79,6 +86,23 @@ def test_null_arguments_are_refused():
         assert "null" in C.lib().tread_last_error().decode()
 
 
+def test_binding_refuses_host_tensors():
+    import torch
+
+    from tread_b200 import kernels
+
+    x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    pages, table, pos = torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2).long()
+    with pytest.raises(ValueError, match="no CPU path"):
+        kernels.paged_append(x, x, pages, pages, table, pos)
+    with pytest.raises(ValueError, match="no CPU path"):
+        kernels.paged_attn(x, pages, pages, table, pos)
+    with pytest.raises(ValueError, match="no CPU path"):
+        kernels.adjust_logits(torch.zeros(2, 5))
+    with pytest.raises(TypeError, match="k_pages must be a tensor"):
+        kernels.paged_attn(x, [1], pages, table, pos)
+
+
 def test_packed_structs_have_the_headers_layout(tmp_path):
     """Sizes and last fields' offsets, as the C compiler lays the structs out."""
     import os
@@ -99,7 +123,7 @@ def test_packed_structs_have_the_headers_layout(tmp_path):
         }""")
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
     got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], capture_output=True, check=True).stdout.split()]
-    append, attn, logits = C.PAGED_APPEND.size, C.PAGED_ATTN.size, C.ADJUST_LOGITS.size
+    append, attn, logits = PAGED_APPEND.size, PAGED_ATTN.size, ADJUST_LOGITS.size
     assert got == [append, append - 8, attn, attn - 4, logits, logits - 8]
 
 

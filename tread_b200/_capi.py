@@ -4,11 +4,13 @@ The library is loaded from the package tree (`tread_b200/_lib/libtread_b200.so`)
 no fallback: if the library is missing or a call fails, a RuntimeError says why.
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
-import struct
 
 import torch
 
+BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "tread_decode.so")
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libtread_b200.so")
 
 TREAD_F32, TREAD_F16, TREAD_BF16 = 0, 1, 2
@@ -69,7 +71,7 @@ SIGNATURES = {
     ),
     "tread_rmsnorm": (ctypes.c_int, [P, I64, P, P, I64, I64, ctypes.c_int, F32, ctypes.c_int, P]),
     "tread_silu_mul": (ctypes.c_int, [P, I64, P, I64, I64, ctypes.c_int, ctypes.c_int, P]),
-    # arguments in a struct: packed by PAGED_APPEND, PAGED_ATTN and ADJUST_LOGITS below
+    # a pointer to the argument struct, and the stream
     "tread_paged_append": (ctypes.c_int, [ctypes.c_char_p, P]),
     "tread_paged_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "tread_paged_attn": (ctypes.c_int, [ctypes.c_char_p, P]),
@@ -81,12 +83,6 @@ SIGNATURES = {
     "tread_kv_spill_rows": (ctypes.c_int, [P, ctypes.c_size_t, P, ctypes.c_size_t, ctypes.c_size_t,
                                            ctypes.c_size_t, P]),
 }
-
-# The fields of the argument structs in order, natively aligned: one struct argument costs about 1 us
-# of host time where thirty ctypes arguments cost 8.
-PAGED_APPEND = struct.Struct("@12P10q8if0q")  # tread_paged_append_args
-PAGED_ATTN = struct.Struct("@8P6q7if")        # tread_paged_attn_args
-ADJUST_LOGITS = struct.Struct("@11P6q6i3f0q")  # tread_adjust_logits_args
 
 _lib = None
 
@@ -105,6 +101,24 @@ def lib():
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """The compiled binding of the decode-step operators (csrc/decode_binding.cpp), loaded once."""
+    global _binding
+    if _binding is None:
+        if not os.path.exists(BINDING_PATH):
+            raise RuntimeError(
+                f"tread_b200 decode binding not built ({BINDING_PATH} missing); run `python -m tread_b200.build`")
+        lib()
+        loader = importlib.machinery.ExtensionFileLoader("tread_decode", BINDING_PATH)
+        spec = importlib.util.spec_from_file_location("tread_decode", BINDING_PATH, loader=loader)
+        _binding = importlib.util.module_from_spec(spec)
+        loader.exec_module(_binding)
+    return _binding
 
 
 def check(rc, what):

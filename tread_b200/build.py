@@ -2,7 +2,9 @@
 
 Every `csrc/*.cu` is compiled with nvcc for `sm_100a` only and linked into one shared
 library with the CUDA runtime linked statically, so the `.so` has no dependency beyond the
-driver. The library is built in-tree so that it travels with the source tree.
+driver. `csrc/decode_binding.cpp`, the Python binding of the decode-step operators, is compiled with
+g++ against PyTorch's headers into `_lib/tread_decode.so` beside it. Both are built in-tree so that
+they travel with the source tree.
 
     python -m tread_b200.build [-v] [--force]
 """
@@ -18,6 +20,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 LIB = os.path.join(OUT_DIR, "libtread_b200.so")
+BINDING = os.path.join(OUT_DIR, "tread_decode.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -66,7 +69,29 @@ def build(verbose=False, force=False, ptxas_verbose=False):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+    src = os.path.join(CSRC, "decode_binding.cpp")
+    if force or _stale(BINDING, [src, os.path.join(ROOT, "include", "tread_b200.h")]):
+        build_binding(src, verbose)
     return LIB
+
+
+def build_binding(src, verbose=False):
+    import sysconfig
+
+    import torch
+
+    root = os.path.join(os.path.dirname(torch.__file__))
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    include = [os.path.join(ROOT, "include"), os.path.join(root, "include"),
+               os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"], cuda]
+    lib = os.path.join(root, "lib")
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{d}" for d in include]
+    cmd += [src, "-o", BINDING, f"-L{OUT_DIR}", f"-L{lib}", "-ltread_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+            "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
 
 
 if __name__ == "__main__":

@@ -474,61 +474,13 @@ def rows_gemm(x, w, bias=None, out=None, accumulate=False, err=None, stream=None
 
 # ---- decode step over a paged cache ---------------------------------------------------------------
 
-# The checks of these wrappers read each shape and stride once and compare device numbers: a decode step
+# These three go through the compiled binding (csrc/decode_binding.cpp), which makes the checks: a decode step
 # makes two such calls a layer, and host time is what bounds it for few sequences.
 
-def _pages(k_pages, v_pages):
-    """(shape, page stride, head stride) of a pair of pools [N, Hkv, page_size, D] with contiguous
-    [page_size, D] planes: a whole pool, or one layer of [N, L, Hkv, page_size, D]."""
-    C.require_cuda(k_pages, "k_pages")
-    shape, stride = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != stride:
-        raise ValueError("k_pages and v_pages must be [pages, Hkv, page_size, D] of one shape and strides")
-    if (stride[3] != 1 or (stride[2] != shape[3] and shape[2] != 1)) or k_pages.dtype != v_pages.dtype:
-        raise ValueError("k_pages and v_pages must share a dtype and have contiguous [page_size, D] planes")
-    return shape, stride[0], stride[1]
-
-
-def _table(table):
-    """(row stride, sequences, pages of a sequence) of a page table."""
-    shape, stride = table.shape, table.stride()
-    if len(shape) != 2 or table.dtype != torch.int32 or (stride[1] != 1 and shape[1] > 1):
-        raise ValueError("table must be int32 [sequences, pages] with unit column stride")
-    return stride[0], shape[0], shape[1]
-
-
-def _index(t, n, dtype, name):
-    if t.shape != (n,) or t.dtype != dtype or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of length {n}")
-
-
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
-
-
-def _elsewhere(index, stream):
-    """The context of a call on tensors of CUDA device `index`: launches and allocations go to the current
-    device and stream."""
-    if stream is None:
-        return torch.cuda.device(index)
-    if stream.device.index != index:
-        raise ValueError(f"the stream is on {stream.device}, the call's tensors on cuda:{index}")
+def _on_stream(stream, t):
+    if t.device != stream.device:
+        raise ValueError(f"the stream is on {stream.device}, the call's tensors on {t.device}")
     return torch.cuda.stream(stream)
-
-
-def _on(t, index, name):
-    if t.get_device() != index:
-        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{index}")
-
-
-def _launch(name, index, args):
-    """Call the library's function `name` with its argument struct on the current stream of a device."""
-    rc = getattr(C.lib(), name)(args, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        C.check(rc, name)
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
 
 
 def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, rope_pos=None, attn_scaling=1.0, q=None,
@@ -547,65 +499,10 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
     err: device error word; a row whose sequence, position or page is out of range appends nothing, gets
       a zero query and sets bit 0.
     Returns the rotated queries [R, Hq, D] (q_out, which may be q itself), or None without q."""
-    (N, Hkv, page_size, D), sp, sh = _pages(k_pages, v_pages)
-    index = k_pages.get_device()
-    if stream is not None or _current_device() != index:
-        with _elsewhere(index, stream):
+    if stream is not None:
+        with _on_stream(stream, k_pages):
             return paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out, err)
-    if not (k.get_device() == v.get_device() == v_pages.get_device() == table.get_device() == pos.get_device() == index):
-        C.same_device(k_pages, k=k, v=v, v_pages=v_pages, table=table, pos=pos)
-    dtype, shape = k.dtype, k.shape
-    k_ld, k_sh, k_last = k.stride() if len(shape) == 3 else (0, 0, 0)
-    if k_last != 1 or shape[1] != Hkv or shape[2] != D or v.shape != shape or v.stride(2) != 1:
-        raise ValueError(f"k and v must be [R, {Hkv}, {D}] with unit last stride")
-    if not (dtype == v.dtype == k_pages.dtype):
-        raise TypeError("k, v and the pages must share a dtype")
-    R = shape[0]
-    v_ld, v_sh, _ = v.stride()
-    ld, S, width = _table(table)
-    at = (R,)
-    if pos.shape != at or pos.dtype != torch.int64 or not pos.is_contiguous():
-        _index(pos, R, torch.int64, "pos")
-    seq_ptr = rope_ptr = inv_ptr = err_ptr = q_ptr = out_ptr = Hq = q_ld = q_sh = 0
-    if seq is not None:
-        _index(seq, R, torch.int32, "seq")
-        _on(seq, index, "seq")
-        seq_ptr = seq.data_ptr()
-    elif R > S:
-        raise ValueError(f"{R} rows without seq, but a table of {S} sequences")
-    if rope_pos is not None:
-        _index(rope_pos, R, torch.int64, "rope_pos")
-        _on(rope_pos, index, "rope_pos")
-        rope_ptr = rope_pos.data_ptr()
-    if inv_freq is not None:
-        _index(inv_freq, D // 2, torch.float32, "inv_freq")
-        _on(inv_freq, index, "inv_freq")
-        inv_ptr = inv_freq.data_ptr()
-    if err is not None:
-        _on(err, index, "err")
-        err_ptr = err.data_ptr()
-    if q is not None:
-        shape = q.shape
-        q_ld, q_sh, q_last = q.stride() if len(shape) == 3 else (0, 0, 0)
-        if q_last != 1 or shape[0] != R or shape[2] != D or q.dtype != dtype:
-            raise ValueError(f"q must be [{R}, Hq, {D}] of k's dtype with unit last stride")
-        if inv_freq is None:
-            raise ValueError("q without inv_freq: nothing rotates it")
-        _on(q, index, "q")
-        if q_out is None:
-            q_out = q.new_empty(shape)
-        elif q_out.shape != shape or q_out.dtype != dtype or not q_out.is_contiguous():
-            raise ValueError(f"q_out must be a contiguous {tuple(shape)} tensor of q's dtype")
-        else:
-            _on(q_out, index, "q_out")
-        Hq, q_ptr, out_ptr = shape[1], q.data_ptr(), q_out.data_ptr()
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    _launch("tread_paged_append", index, C.PAGED_APPEND.pack(
-        k.data_ptr(), v.data_ptr(), q_ptr, out_ptr, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), seq_ptr,
-        pos.data_ptr(), rope_ptr, inv_ptr, err_ptr, k_ld, k_sh, v_ld, v_sh, q_ld, q_sh, sp, sh, N, ld, page_size, S, width,
-        R, Hq, Hkv, D, C.dtype_code(dtype), attn_scaling))
-    return q_out
+    return C.binding().paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out, err)
 
 
 def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=None, stream=None):
@@ -615,57 +512,10 @@ def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=No
     has a score above -inf, or there is none (length 0), the output is zero.
     err: device error word; a length that the table has no pages for gives a row of zeros and sets bit
     1, and so does a page id outside the pool, whose keys count as masked. Returns out [B, Hq, D]."""
-    (N, Hkv, page_size, D), sp, sh = _pages(k_pages, v_pages)
-    index = k_pages.get_device()
-    if stream is not None or _current_device() != index:
-        with _elsewhere(index, stream):
+    if stream is not None:
+        with _on_stream(stream, k_pages):
             return paged_attn(q, k_pages, v_pages, table, lens, out, sm_scale, err)
-    if not (q.get_device() == v_pages.get_device() == table.get_device() == lens.get_device() == index):
-        C.same_device(k_pages, q=q, v_pages=v_pages, table=table, lens=lens)
-    shape, stride, dtype = q.shape, q.stride(), q.dtype
-    if len(shape) != 3 or shape[2] != D or stride[2] != 1 or (shape[1] > 1 and stride[1] != D) or dtype != k_pages.dtype:
-        raise ValueError(f"q must be [B, Hq, {D}] of the pages' dtype with contiguous rows")
-    B, Hq, _ = shape
-    ld, S, width = _table(table)
-    if S != B:
-        raise ValueError(f"table must have a row for each of the {B} sequences")
-    _index(lens, B, torch.int64, "lens")
-    if out is None:
-        out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype != dtype or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {tuple(shape)} tensor of q's dtype")
-    else:
-        _on(out, index, "out")
-    err_ptr = 0
-    if err is not None:
-        _on(err, index, "err")
-        err_ptr = err.data_ptr()
-    # one workspace a call, from the allocator: calls of several streams, threads and graphs share none
-    nbytes = C.lib().tread_paged_attn_workspace_bytes(Hq, Hkv, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    _launch("tread_paged_attn", index, C.PAGED_ATTN.pack(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), err_ptr,
-        ws.data_ptr(), stride[0], sp, sh, N, ld, nbytes, page_size, width, B, Hq, Hkv, D, C.dtype_code(dtype),
-        D ** -0.5 if sm_scale is None else sm_scale))
-    return out
-
-
-def _per_row(x, B, name, index):
-    """A penalty as (device pointer or 0, value for all rows)."""
-    if isinstance(x, torch.Tensor):
-        if x.get_device() != index:
-            raise ValueError(f"{name} is on {x.device}, the logits on cuda:{index}")
-        _index(x, B, torch.float32, name)
-        return x.data_ptr(), 1.0
-    return 0, float(x)
-
-
-def _by_row(t, B, width, dtype, name):
-    """Row stride of t [B, width], or 0 for one row [width] that serves every row."""
-    shape, stride = t.shape, t.stride()
-    if t.dtype != dtype or not (shape == (B, width) or shape == (width,)) or (width > 1 and stride[-1] != 1):
-        raise ValueError(f"{name} must be {dtype} [{B}, {width}] or [{width}] with unit last stride")
-    return stride[0] if len(shape) == 2 else 0
+    return C.binding().paged_attn(q, k_pages, v_pages, table, lens, out, sm_scale, err)
 
 
 def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1.0, presence=0.0, frequency=0.0,
@@ -683,58 +533,12 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
       -inf where the grammar does not allow it: bit v % 32 of allowed[..., v // 32] (int32 [B, W], or
       [W] for all rows, W = ceil(V / 32)) is 0.
     Returns out: fp32 [B, V] by default; a given one may be of any supported dtype, or logits itself."""
-    C.require_cuda(logits, "logits")
-    index = logits.get_device()
-    if stream is not None or _current_device() != index:
-        with _elsewhere(index, stream):
-            return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
-                                 allowed, out)
-    shape, stride = logits.shape, logits.stride()
-    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
-        raise ValueError("logits must be [B, V] with unit column stride")
-    B, V = shape
-    for t in (tokens, lens, prompt_lens, bias_ids, bias, allowed, out):
-        if t is not None and t.get_device() != index:
-            C.same_device(logits, tokens=tokens, lens=lens, prompt_lens=prompt_lens, bias_ids=bias_ids, bias=bias,
-                          allowed=allowed, out=out)
-    H = tok_ld = 0
-    if tokens is not None:
-        t_shape, t_stride = tokens.shape, tokens.stride()
-        if len(t_shape) != 2 or t_shape[0] != B or tokens.dtype != torch.int64 or (t_shape[1] > 1 and t_stride[1] != 1):
-            raise ValueError(f"tokens must be int64 [{B}, H] with unit column stride")
-        H, tok_ld = t_shape[1], t_stride[0]
-        if lens is not None:
-            _index(lens, B, torch.int64, "lens")
-        if prompt_lens is not None:
-            _index(prompt_lens, B, torch.int64, "prompt_lens")
-    elif lens is not None or prompt_lens is not None:
-        raise ValueError("lens and prompt_lens without tokens")
-    rep, rep_all = _per_row(repetition, B, "repetition", index)
-    pres, pres_all = _per_row(presence, B, "presence", index)
-    freq, freq_all = _per_row(frequency, B, "frequency", index)
-    if not rep_all > 0:
-        raise ValueError(f"repetition must be above 0, got {repetition}")
-    nb = ids_ld = bias_ld = 0
-    if (bias is None) != (bias_ids is None):
-        raise ValueError("bias and bias_ids come together")
-    if bias is not None:
-        nb = bias_ids.shape[-1]
-        ids_ld, bias_ld = _by_row(bias_ids, B, nb, torch.int64, "bias_ids"), _by_row(bias, B, nb, torch.float32, "bias")
-    allowed_ld = 0 if allowed is None else _by_row(allowed, B, (V + 31) // 32, torch.int32, "allowed")
-    if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=logits.device)
-        out_ld = V
-    else:
-        out_ld, *last = out.stride()
-        if out.shape != shape or (V > 1 and last != [1]):
-            raise ValueError(f"out must be [{B}, {V}] with unit column stride")
-        if out.data_ptr() == logits.data_ptr() and (out.dtype != logits.dtype or out_ld != stride[0]):
-            raise ValueError("out over logits must have their dtype and row stride")
-    _launch("tread_adjust_logits", index, C.ADJUST_LOGITS.pack(
-        logits.data_ptr(), out.data_ptr(), _ptr(tokens), _ptr(lens), _ptr(prompt_lens), rep, pres, freq, _ptr(bias_ids),
-        _ptr(bias), _ptr(allowed), stride[0], out_ld, tok_ld, ids_ld, bias_ld, allowed_ld, B, V, H, nb,
-        C.dtype_code(logits.dtype), C.dtype_code(out.dtype), rep_all, pres_all, freq_all))
-    return out
+    if stream is not None:
+        with _on_stream(stream, logits):
+            return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, allowed,
+                                 out)
+    return C.binding().adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
+                                     allowed, out)
 
 
 # ---- fused row-wise layer pieces ----------------------------------------------------------------
