@@ -331,7 +331,7 @@ int tread_paged_attn(const tread_paged_attn_args* args, tread_stream_t stream);
  *                 (repetition above 0)
  *   bias_ids, bias: device int64 / fp32 [B, num_bias] at their row strides (0: one list for all rows);
  *                 ids outside [0, V) count for nothing, several biases of one token add up in order;
- *                 num_bias at most 4096
+ *                 num_bias at most 2048
  *   allowed     : device int32 [B, ceil(V / 32)] at row stride allowed_ld (0: one mask for all rows),
  *                 bit v % 32 of word v / 32 set: v is allowed; NULL: every token is
  */

@@ -172,6 +172,24 @@ def test_shared_memory_of_every_size(H):
     _check(got[few], logits[few], **{k: v[few] for k, v in kw.items()})
 
 
+@pytest.mark.parametrize("H", [9000, 20000])
+@pytest.mark.parametrize("where", ["new", "in place"])
+def test_more_changed_tokens_than_a_slice_has_room_for(H, where):
+    """Histories of thousands of different tokens side by side, with biases among them."""
+    B, V = 64, 152064
+    logits, kw = _case(B, V, H, BF, H, biases=300)
+    g = _gen(H + 1)
+    kw["tokens"] = torch.randint(0, 16000, (B, H), device=DEV, generator=g)
+    kw["bias_ids"] = torch.randint(0, 17000, (B, 300), device=DEV, generator=g)
+    kw["lens"][:3] = H
+    kw["prompt_lens"][0] = H
+    kw["allowed"][1] = -1
+    few = slice(0, 3)
+    before = logits[few].clone()
+    got = kernels.adjust_logits(logits, out=logits if where == "in place" else None, **kw)
+    _check(got[few], before, **{k: v[few] for k, v in kw.items()})
+
+
 def test_graph_replay_and_streams():
     logits, kw = _case(4, 20000, 100, BF, 14)
     want = kernels.adjust_logits(logits, **kw)

@@ -71,7 +71,7 @@ def _logits_call(**over):
 @pytest.mark.parametrize("over,needle", [
     (dict(B=-1), "B < 0"), (dict(x=None), "null"), (dict(out=None), "null"), (dict(dtype=5), "dtype"),
     (dict(odt=5), "dtype"), (dict(ld=99), "row stride"), (dict(ld_out=99), "row stride"), (dict(H=-1), "history"),
-    (dict(tok_ld=7), "history"), (dict(H=2 ** 30 + 1, tok_ld=2 ** 31), "history"), (dict(bias=None), "biases"), (dict(nb=-1), "biases"), (dict(nb=4097), "4096 biases"),
+    (dict(tok_ld=7), "history"), (dict(H=2 ** 30 + 1, tok_ld=2 ** 31), "history"), (dict(bias=None), "biases"), (dict(nb=-1), "biases"), (dict(nb=2049), "2048 biases"),
     (dict(B=65536), "65535 rows"), (dict(V=2 ** 31 - 1, ld=2 ** 31, ld_out=2 ** 31), "rows"), (dict(rep_all=0.0), "repetition"),
     (dict(rep_all=float("nan")), "repetition"),
 ])

@@ -6,30 +6,29 @@
 //   x -= frequency * n[v] + presence * (n[v] > 0);   x += bias of v;   v not allowed: x = -inf
 // in fp32, rounded once to the output's type. Ids outside [0, vocab) count for nothing (padding).
 //
-// Bound by reading the logits and writing the result. A CTA owns a slice of a row's vocabulary. Half of its
-// warps store every logit of the slice, masked, in vectors; the other half meanwhile count the row's whole
-// history into counters of the slice in shared memory (whole numbers: the order of the atomics does not
-// matter). Then all of them finish the few tokens that the history or a bias changes. One after the other,
-// the history's latency left the memory idle for as long as the logits took.
+// Bound by reading the logits and writing the result. A CTA owns a slice of a row's vocabulary and issues its
+// first loads. While they fly it counts the row's whole history into counters of the slice in shared memory
+// (whole numbers: the order of the atomics does not matter), and computes the slice's few biased tokens, each by
+// the thread that marked it first. Then one pass reads, penalises, masks and stores every logit, and the biased
+// ones are stored again. The penalties' instructions, which nearly every warp goes through for one of its
+// 256 tokens, fit under the memory's time; finishing the history's tokens by themselves did not: scattered
+// reads of their logits take 7 us before the pass, and reads and writes in place 13 us after it (64 rows of
+// 152064, histories of up to 8768).
 // Reading the history again for every slice costs L2 reads only, and no counters in memory that a caller would
 // have to keep or clear. A warp that looks at 32 ids meets one of its slice nearly every time, so ids are only
-// sorted out there, and the slice's own are queued until 32 lanes have one each; tokens are listed when their
-// counters are first touched, and finished by whole warps. A biased token is finished by the thread that
-// marked it first.
+// sorted out there, and the slice's own are queued until 32 lanes have one each.
 #include "common.cuh"
 
 namespace tread {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kStreaming = 128;  // of them; the rest go through the history
-constexpr int kCounting = kThreads - kStreaming;
 constexpr int kMaxSlice = 18432;
 constexpr int kCtas = 4;         // CTAs of an SM
 constexpr int kVec = 8;          // consecutive logits of a thread
-constexpr int kQueue = 512;      // tokens of the slice that a warp gathers from the history
+constexpr int kQueue = 288;      // tokens of the slice that a warp gathers from the history
 constexpr int kQueuePrompt = 1 << 15;
-constexpr int kMaxBias = 4096;   // 32 bits of ownership a thread
+constexpr int kMaxBias = 2048;   // biases of a row: their values' room in shared memory
 
 using LogitsArgs = tread_adjust_logits_args;
 
@@ -40,7 +39,6 @@ struct Counter {
   static constexpr unsigned kPrompt = 1u << (kBits - 1);  // the prompt holds it
   static constexpr unsigned kBiased = 1u << (kBits - 2);
   static constexpr unsigned kCount = kBiased - 1;
-  static constexpr unsigned kAll = kPrompt | kBiased | kCount;
   // marks or counts token i of the slice; returns its counter as it was
   static __device__ __forceinline__ unsigned mark(W* c, int i, unsigned what) {
     if constexpr (sizeof(W) == 4) return atomicOr(reinterpret_cast<unsigned*>(c) + i, what);
@@ -76,17 +74,16 @@ __device__ __forceinline__ void store8(void* out, long long i, const float (&x)[
   }
 }
 
-// VECS: vectors of kVec logits that a streaming thread has in flight
+// VECS: vectors of kVec logits that a thread has in flight
 template <typename T, typename W, int VECS>
 __global__ void __launch_bounds__(kThreads, kCtas)
     adjust_logits_kernel(const __grid_constant__ LogitsArgs a, int slice) {
   using C = Counter<W>;
   extern __shared__ __align__(16) unsigned char s_mem[];
-  __shared__ int s_twice;                  // some token of the slice has more than one bias
-  __shared__ int s_listed;
-  __shared__ uint16_t s_queue[kCounting / 32][kQueue];
+  __shared__ int s_twice;   // some token of the slice has more than one bias
+  __shared__ uint16_t s_queue[kThreads / 32][kQueue];
+  __shared__ float s_value[kMaxBias];
   W* count = reinterpret_cast<W*>(s_mem);  // of tokens first - kVec .. first + slice - 1
-  uint16_t* list = reinterpret_cast<uint16_t*>(count + slice + kVec);  // the history's tokens, once each
   const int b = blockIdx.y;
   const T* row = static_cast<const T*>(a.logits) + b * a.ld;
   const long long out_row = b * a.ld_out;
@@ -101,111 +98,41 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   const int tid = threadIdx.x;
   const unsigned* allowed = a.allowed ? reinterpret_cast<const unsigned*>(a.allowed) + b * a.allowed_ld : nullptr;
   auto is_allowed = [&](int v) { return !allowed || (allowed[v >> 5] >> (v & 31)) & 1; };
+  constexpr int L = kVec * sizeof(T) / 16;  // 16-byte loads of a vector
+  int4 x[VECS][L];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+      const int i = i0 + k * kThreads;
+      if (i < vecs) {
+#pragma unroll
+        for (int j = 0; j < L; ++j) x[k][j] = ld_stream(row + first + i * kVec + j * (16 / sizeof(T)));
+      }
+    }
+  };
+  load(tid);
+  const bool changes = a.tokens || a.num_bias;
+  const float rep = a.repetition ? a.repetition[b] : a.repetition_all;
+  const float pres = a.presence ? a.presence[b] : a.presence_all;
+  const float freq = a.frequency ? a.frequency[b] : a.frequency_all;
+  // x / repetition as a product with its reciprocal: a rounding more, a division's dozen instructions fewer;
+  // but for reciprocals that overflow or lose digits
+  const float inv = 1.f / rep;
+  const bool product = rep > 0x1p-100f && rep < 0x1p100f;
+  auto penalised = [&](float f, unsigned c) {  // c: not 0
+    f = f > 0.f ? (product ? f * inv : f / rep) : f * rep;
+    const unsigned n = c & C::kCount;
+    return n ? f - (freq * (float)n + pres) : f;
+  };
   unsigned mine = 0;  // biases whose token this thread marked first
   const int64_t* bias_ids = a.bias_ids + b * a.bias_ids_ld;
   const float* bias = a.bias + b * a.bias_ld;
-  if (tid < kStreaming) {
-    constexpr int L = kVec * sizeof(T) / 16;  // 16-byte loads of a vector
-    const bool aligned =
-        (reinterpret_cast<uintptr_t>(a.out) + (out_row + first) * (a.out_dtype == TREAD_F32 ? 4 : 2)) % 16 == 0;
-    for (int i0 = tid; i0 < vecs; i0 += VECS * kStreaming) {
-      int4 x[VECS][L];
-#pragma unroll
-      for (int k = 0; k < VECS; ++k) {
-        const int i = i0 + k * kStreaming;
-        if (i < vecs) {
-#pragma unroll
-          for (int j = 0; j < L; ++j) x[k][j] = ld_stream(row + first + i * kVec + j * (16 / sizeof(T)));
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < VECS; ++k) {
-        const int i = i0 + k * kStreaming;
-        if (i >= vecs) continue;
-        const int v = first + i * kVec;
-        float f[kVec];
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          Vec16<T> u;
-          u.raw = x[k][e * sizeof(T) / 16];
-          f[e] = Num<T>::to_f(u.e[e % (16 / sizeof(T))]);
-        }
-        if (allowed) {
-          const int shift = v & 31;
-          unsigned bits = allowed[v >> 5] >> shift;
-          if (shift > 32 - kVec) bits |= allowed[(v >> 5) + 1] << (32 - shift);
-#pragma unroll
-          for (int e = 0; e < kVec; ++e)
-            if (!((bits >> e) & 1)) f[e] = -INFINITY;
-        }
-        if (!aligned) {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) store(a.out, out_row + v + e, a.out_dtype, f[e]);
-        } else if (a.out_dtype == TREAD_F32) {
-          store8<float>(a.out, out_row + v, f);
-        } else if (a.out_dtype == TREAD_BF16) {
-          store8<__nv_bfloat16>(a.out, out_row + v, f);
-        } else {
-          store8<__half>(a.out, out_row + v, f);
-        }
-      }
-    }
-    // the first slice's tokens before its vectors (a short row may have no others), and the row's last ones
-    auto single = [&](int v) { store(a.out, out_row + v, a.out_dtype, is_allowed(v) ? Num<T>::to_f(row[v]) : -INFINITY); };
-    if (tid < min(first, end) - begin) single(begin + tid);
-    if (tid < end - first - vecs * kVec) single(first + vecs * kVec + tid);
-  } else if (a.tokens || a.num_bias) {
-    const int lane = tid & 31, me = tid - kStreaming;
-    for (int i = me; i < (int)((slice + kVec) * sizeof(W) / 16); i += kCounting)
+  if (changes) {
+    for (int i = tid; i < (int)((slice + kVec) * sizeof(W) / 16); i += kThreads)
       reinterpret_cast<int4*>(s_mem)[i] = make_int4(0, 0, 0, 0);
-    if (me == 0) s_twice = s_listed = 0;
-    asm volatile("bar.sync 1, %0;" ::"n"(kCounting) : "memory");
-    long long len = !a.tokens ? 0 : a.lens ? a.lens[b] : a.max_tokens;
-    len = len < 0 ? 0 : len > a.max_tokens ? a.max_tokens : len;
-    const long long prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
-    const long long* ids = reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_ld;
-    uint16_t* queue = s_queue[me >> 5];
-    int queued = 0;  // the same in all lanes
-    auto count_queued = [&]() {
-      __syncwarp();
-      for (int j = 0; j < queued; j += 32) {
-        bool fresh = false;
-        int at = 0;
-        if (j + lane < queued) {
-          at = queue[j + lane] & (kQueuePrompt - 1);
-          const unsigned was = queue[j + lane] & kQueuePrompt ? C::mark(count, at, C::kPrompt) : C::add(count, at);
-          fresh = !(was & C::kAll);
-        }
-        const unsigned who = __ballot_sync(0xffffffffu, fresh);
-        int to = 0;
-        if (lane == 0 && who) to = atomicAdd(&s_listed, __popc(who));
-        to = __shfl_sync(0xffffffffu, to, 0);
-        if (fresh) list[to + __popc(who & ((1u << lane) - 1))] = (uint16_t)at;
-      }
-      __syncwarp();
-      queued = 0;
-    };
-    constexpr int kAhead = 8;
-    for (int i0 = me - lane; i0 < (int)len; i0 += kCounting * kAhead) {
-      long long v[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = i0 + lane + k * kCounting;
-        v[k] = i < (int)len ? __ldg(ids + i) : -1;
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const bool hit = v[k] >= begin && v[k] < end;
-        const unsigned who = __ballot_sync(0xffffffffu, hit);
-        if (hit)
-          queue[queued + __popc(who & ((1u << lane) - 1))] =
-              (uint16_t)(((int)v[k] - origin) | (i0 + lane + k * kCounting < prompt ? kQueuePrompt : 0));
-        queued += __popc(who);
-      }
-      if (queued > kQueue - 32 * kAhead) count_queued();
-    }
-    count_queued();
-    for (int i = me, k = 0; i < a.num_bias; i += kCounting, ++k) {
+    if (tid == 0) s_twice = 0;
+    __syncthreads();
+    for (int i = tid, k = 0; i < a.num_bias; i += kThreads, ++k) {
       const long long v = bias_ids[i];
       if (v < begin || v >= end) continue;
       if (C::mark(count, (int)v - origin, C::kBiased) & C::kBiased)
@@ -213,39 +140,127 @@ __global__ void __launch_bounds__(kThreads, kCtas)
       else
         mine |= 1u << k;
     }
-  }
-  if (!a.tokens && !a.num_bias) return;
-  // behind all stores; where out is logits, an allowed token still has its logit
-  __syncthreads();
-  const float rep = a.repetition ? a.repetition[b] : a.repetition_all;
-  const float pres = a.presence ? a.presence[b] : a.presence_all;
-  const float freq = a.frequency ? a.frequency[b] : a.frequency_all;
-  auto penalised = [&](float f, unsigned c) {
-    if (c & ~C::kBiased) {
-      f = f > 0.f ? f / rep : f * rep;
-      if (c & C::kCount) f -= freq * (float)(c & C::kCount) + pres;
+    if (a.tokens) {
+      const int lane = tid & 31;
+      long long len = a.lens ? a.lens[b] : a.max_tokens;
+      len = len < 0 ? 0 : len > a.max_tokens ? a.max_tokens : len;
+      const long long prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
+      const long long* ids = reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_ld;
+      uint16_t* queue = s_queue[tid >> 5];
+      int queued = 0;  // the same in all lanes
+      auto count_queued = [&]() {
+        __syncwarp();
+        for (int j = 0; j < queued; j += 32) {
+          if (j + lane >= queued) continue;
+          const int at = queue[j + lane] & (kQueuePrompt - 1);
+          if (queue[j + lane] & kQueuePrompt)
+            C::mark(count, at, C::kPrompt);
+          else
+            C::add(count, at);
+        }
+        __syncwarp();
+        queued = 0;
+      };
+      constexpr int kAhead = 8;
+      for (int i0 = tid - lane; i0 < (int)len; i0 += kThreads * kAhead) {
+        long long v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = i0 + lane + k * kThreads;
+          v[k] = i < (int)len ? __ldg(ids + i) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const bool hit = v[k] >= begin && v[k] < end;
+          const unsigned who = __ballot_sync(0xffffffffu, hit);
+          if (hit)
+            queue[queued + __popc(who & ((1u << lane) - 1))] =
+                (uint16_t)(((int)v[k] - origin) | (i0 + lane + k * kThreads < prompt ? kQueuePrompt : 0));
+          queued += __popc(who);
+        }
+        if (queued > kQueue - 32 * kAhead) count_queued();
+      }
+      count_queued();
     }
-    return f;
+    __syncthreads();
+    // the biased tokens, biases added up in the list's order
+    for (int k = 0; mine >> k; ++k) {
+      if (!((mine >> k) & 1)) continue;
+      const int i = k * kThreads + tid, v = (int)bias_ids[i];
+      const unsigned c = count[v - origin] & ~C::kBiased;
+      float sum = bias[i];
+      if (s_twice) {
+        sum = 0.f;
+        for (int j = 0; j < a.num_bias; ++j)
+          if (bias_ids[j] == v) sum += bias[j];
+      }
+      const float f = Num<T>::to_f(row[v]);
+      s_value[i] = is_allowed(v) ? (c ? penalised(f, c) : f) + sum : -INFINITY;
+    }
+    if (a.num_bias) __syncthreads();  // their logits are read before the pass writes them, where out is logits
+  }
+  // the pass
+  const bool aligned =
+      (reinterpret_cast<uintptr_t>(a.out) + (out_row + first) * (a.out_dtype == TREAD_F32 ? 4 : 2)) % 16 == 0;
+  for (int i0 = tid; i0 < vecs; i0 += VECS * kThreads) {
+    if (i0 != tid) load(i0);
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+      const int i = i0 + k * kThreads;
+      if (i >= vecs) continue;
+      const int v = first + i * kVec;
+      float f[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        Vec16<T> u;
+        u.raw = x[k][e * sizeof(T) / 16];
+        f[e] = Num<T>::to_f(u.e[e % (16 / sizeof(T))]);
+      }
+      if (changes) {
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(W) / 2; ++j) {
+          constexpr int E = 16 / sizeof(W);
+          Vec16<W> c;
+          c.raw = reinterpret_cast<const int4*>(count + (i + 1) * kVec)[j];
+          if (c.raw.x | c.raw.y | c.raw.z | c.raw.w) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (c.e[e]) f[j * E + e] = penalised(f[j * E + e], c.e[e]);
+          }
+        }
+      }
+      if (allowed) {
+        const int shift = v & 31;
+        unsigned bits = allowed[v >> 5] >> shift;
+        if (shift > 32 - kVec) bits |= allowed[(v >> 5) + 1] << (32 - shift);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (!((bits >> e) & 1)) f[e] = -INFINITY;
+      }
+      if (!aligned) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) store(a.out, out_row + v + e, a.out_dtype, f[e]);
+      } else if (a.out_dtype == TREAD_F32) {
+        store8<float>(a.out, out_row + v, f);
+      } else if (a.out_dtype == TREAD_BF16) {
+        store8<__nv_bfloat16>(a.out, out_row + v, f);
+      } else {
+        store8<__half>(a.out, out_row + v, f);
+      }
+    }
+  }
+  // the first slice's tokens before its vectors (a short row may have no others), and the row's last ones
+  auto single = [&](int v) {
+    const float f = Num<T>::to_f(row[v]);
+    const unsigned c = changes ? count[v - origin] : 0;
+    store(a.out, out_row + v, a.out_dtype, is_allowed(v) ? (c ? penalised(f, c) : f) : -INFINITY);
   };
-  for (int i = tid; i < s_listed; i += kThreads) {
-    const int v = origin + list[i];
-    const unsigned c = count[v - origin];
-    if ((c & C::kBiased) || !is_allowed(v)) continue;
-    store(a.out, out_row + v, a.out_dtype, penalised(Num<T>::to_f(row[v]), c));
-  }
-  for (int k = 0; k < 32 && (mine >> k); ++k) {
-    if (!((mine >> k) & 1)) continue;
-    const int i = k * kCounting + tid - kStreaming;
-    const int v = (int)bias_ids[i];
-    float sum = bias[i];
-    if (s_twice) {
-      sum = 0.f;
-      for (int j = 0; j < a.num_bias; ++j)
-        if (bias_ids[j] == v) sum += bias[j];
-    }
-    store(a.out, out_row + v, a.out_dtype,
-          is_allowed(v) ? penalised(Num<T>::to_f(row[v]), count[v - origin]) + sum : -INFINITY);
-  }
+  if (tid < min(first, end) - begin) single(begin + tid);
+  if (tid < end - first - vecs * kVec) single(first + vecs * kVec + tid);
+  if (!a.num_bias) return;
+  __syncthreads();
+  for (int k = 0; mine >> k; ++k)
+    if ((mine >> k) & 1) store(a.out, out_row + bias_ids[k * kThreads + tid], a.out_dtype, s_value[k * kThreads + tid]);
 }
 
 template <typename T, typename W, int VECS>
@@ -259,9 +274,9 @@ int launch(const LogitsArgs& a, cudaStream_t st) {
   const int most = (int)(((long long)a.V + kPass - 1) / kPass), least = (a.V + kMaxSlice - 1) / kMaxSlice;
   slices = slices > most ? most : slices < least ? least : slices;
   const int slice = (((a.V + slices - 1) / slices) + 63) / 64 * 64;  // whole vectors of counters
-  const int smem = (slice + kVec) * (int)sizeof(W) + (slice < a.max_tokens ? slice : a.max_tokens) * 2 + kVec * 2;
+  const int smem = (slice + kVec) * (int)sizeof(W);
   auto kern = adjust_logits_kernel<T, W, VECS>;
-  if (smem > 32 * 1024) TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 24 * 1024) TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kern<<<dim3(slices, a.B), kThreads, smem, st>>>(a, slice);
   TREAD_CHECK_LAUNCH("adjust_logits_kernel");
   return TREAD_OK;
@@ -295,8 +310,8 @@ extern "C" int tread_adjust_logits(const tread_adjust_logits_args* args, tread_s
   if (!a.tokens) a.max_tokens = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (a.dtype) {
-    case TREAD_BF16: return dispatch<__nv_bfloat16, 4>(a, st);
-    case TREAD_F16: return dispatch<__half, 4>(a, st);
+    case TREAD_BF16: return dispatch<__nv_bfloat16, 3>(a, st);
+    case TREAD_F16: return dispatch<__half, 3>(a, st);
     default: return dispatch<float, 2>(a, st);
   }
 }
