@@ -91,8 +91,8 @@ def test_binding_refuses_host_tensors():
 
     from tread_b200 import kernels
 
-    x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
-    pages, table, pos = torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2).long()
+    x, pages = torch.zeros(2, 2, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16)
+    table, pos = torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int64)
     with pytest.raises(ValueError, match="no CPU path"):
         kernels.paged_append(x, x, pages, pages, table, pos)
     with pytest.raises(ValueError, match="no CPU path"):

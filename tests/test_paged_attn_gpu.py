@@ -167,6 +167,15 @@ def test_shared_pages_and_repeated_calls_give_the_same_bits():
         assert torch.equal(kernels.paged_attn(q, kp, vp, table, lens), got)
 
 
+def test_output_over_the_queries():
+    """out = q: every query is read before its row is written, in shares of one item and of several."""
+    for lens in ([8000, 3], [60] * 100, [0, 5, 700]):
+        q, *rest = _case(lens, 28, 4, 128, 64, BF, 21)
+        want = kernels.paged_attn(q, *rest)
+        got = kernels.paged_attn(q, *rest, out=q)
+        assert got is q and torch.equal(q, want)
+
+
 def test_other_streams_and_graphs():
     """Two graphs with calls of different sizes, and an eager call, each on a stream of its own, replayed
     together again and again."""
@@ -231,6 +240,7 @@ def test_attn_refuses_bad_tensors():
     with pytest.raises(RuntimeError, match="16-byte"):
         kernels.paged_attn(q, off, vp, table, lens)
     with pytest.raises(RuntimeError, match="16-byte"):
-        kernels.paged_attn(torch.empty(2, 4 * 64 + 1, dtype=BF, device=DEV)[:, :256].unflatten(1, (4, 64)), kp, vp, table, lens)
+        odd = torch.empty(2, 4 * 64 + 1, dtype=BF, device=DEV)[:, :256].unflatten(1, (4, 64))
+        kernels.paged_attn(odd, kp, vp, table, lens)
     with pytest.raises(RuntimeError, match="head_dim"):
         kernels.paged_attn(q[..., :32].contiguous(), kp[..., :32].contiguous(), vp[..., :32].contiguous(), table, lens)

@@ -71,7 +71,8 @@ def test_a_batch_of_lengths_equals_each_alone(setup, graphs):
     model, eng = setup
     dec = PagedDecoder(model, num_pages=300, page_size=16, max_seqs=8, max_len=600, graphs=graphs)
     alone = PagedDecoder(model, num_pages=300, page_size=64, max_seqs=8, max_len=600)
-    requests = [_request(eng, 10 + i, lens)[1] for i, lens in enumerate([(9, 40, 33, 7), (5, 3), (60, 200, 100, 30), (16, 16, 16)])]
+    lengths = [(9, 40, 33, 7), (5, 3), (60, 200, 100, 30), (16, 16, 16)]
+    requests = [_request(eng, 10 + i, lens)[1] for i, lens in enumerate(lengths)]
     seqs, solo = [dec.admit(c) for c in requests], [alone.admit(c) for c in requests]
     g = torch.Generator().manual_seed(3)
     for members in ([0, 1, 2, 3], [0, 1, 2, 3], [2, 0], [1], [3, 1, 0], [0, 1, 2, 3]):
@@ -199,8 +200,8 @@ def test_server_with_a_paged_decoder_answers_as_the_reference():
 def test_server_adjusts_logits(decoder):
     g = golden("server.npz")
     client, dec = _client(g, decoder)
-    base = dict(prefix="You are a careful assistant. ", documents=["alpha doc about rivers and lakes"], suffix="Q: which?",
-                max_tokens=8, recompute_ratio=0.0)
+    base = dict(prefix="You are a careful assistant. ", documents=["alpha doc about rivers and lakes"],
+                suffix="Q: which?", max_tokens=8, recompute_ratio=0.0)
     ask = lambda **kw: client.post("/v1/completions", json={**base, **kw})  # noqa: E731
     plain = ask().json()["text"].split()
     assert ask(repetition_penalty=1.0, logit_bias={}, allowed_token_ids=None).json()["text"].split() == plain
@@ -213,11 +214,26 @@ def test_server_adjusts_logits(decoder):
     once = ask(presence_penalty=100.0, max_tokens=16).json()["text"].split()
     assert len(set(once)) == len(once) == 16
     assert ask(repetition_penalty=1.3, frequency_penalty=0.4).status_code == 200
-    for bad in (dict(repetition_penalty=0.0), dict(logit_bias={"4096": 1.0}), dict(allowed_token_ids=[-1]),
+    for bad in (dict(repetition_penalty=0.0), dict(repetition_penalty=1e-50), dict(logit_bias={"4096": 1.0}), dict(allowed_token_ids=[-1]),
                 dict(allowed_token_ids=[]), dict(logit_bias={"x": 1.0}), dict(logit_bias={"1": 1e9})):
         assert ask(**bad).status_code == 422, bad
     if dec is not None:
         assert dec.cache.lens == {}
+
+
+def test_server_without_a_free_page_answers_503():
+    """The decoder's pages are held by another user of it: the request fails, nothing leaks, and the next one
+    works."""
+    client, dec = _client(golden("server.npz"))
+    body = dict(prefix="You are a careful assistant. ", documents=["alpha doc"], suffix="Q: which?", max_tokens=4)
+    held = dec.cache.new(500)
+    more = dec.cache.new(100)
+    assert client.post("/v1/completions", json=body).status_code == 503
+    assert sorted(dec.cache.lens) == sorted([held, more])
+    dec.release(held)
+    dec.release(more)
+    assert client.post("/v1/completions", json=body).status_code == 200
+    assert dec.cache.lens == {}
 
 
 def test_server_refuses_a_decoder_that_is_too_small():

@@ -80,15 +80,15 @@ def build_binding(src, verbose=False):
 
     import torch
 
-    root = os.path.join(os.path.dirname(torch.__file__))
+    root = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
     include = [os.path.join(ROOT, "include"), os.path.join(root, "include"),
                os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"], cuda]
     lib = os.path.join(root, "lib")
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{d}" for d in include]
-    cmd += [src, "-o", BINDING, f"-L{OUT_DIR}", f"-L{lib}", "-ltread_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
-            "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    cmd += [src, "-o", BINDING, f"-L{OUT_DIR}", f"-L{lib}", "-ltread_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+            "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)

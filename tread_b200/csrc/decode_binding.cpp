@@ -31,14 +31,15 @@ int dtype_code(const Tensor& t, const char* name) {
     case at::kBFloat16: return TREAD_BF16;
     case at::kHalf: return TREAD_F16;
     case at::kFloat: return TREAD_F32;
-    default: TORCH_CHECK_TYPE(false, name, ": unsupported dtype ", t.scalar_type(), "; expected float32, float16 or bfloat16");
+    default:
+      TORCH_CHECK_TYPE(false, name, ": unsupported dtype ", t.scalar_type(), "; expected float32, float16 or bfloat16");
   }
 }
 
 // every tensor of a call sits on one device: the kernels dereference them all there
 void on(const Tensor& t, c10::DeviceIndex index, const char* name) {
-  TORCH_CHECK_VALUE(t.is_cuda() && t.get_device() == index, name, " is on ", t.device(), ", the call's other tensors on cuda:",
-                    (int)index);
+  TORCH_CHECK_VALUE(t.is_cuda() && t.get_device() == index, name, " is on ", t.device(),
+                    ", the call's other tensors on cuda:", (int)index);
 }
 
 c10::DeviceIndex device_of(const Tensor& t, const char* name) {
@@ -107,8 +108,9 @@ PyObject* paged_append(PyObject*, PyObject* const* arg, Py_ssize_t count) {
   const auto index = device_of(kp, "k_pages");
   const Pools p = pools(kp, vp);
   on(vp, index, "v_pages"), on(k, index, "k"), on(v, index, "v");
-  TORCH_CHECK_VALUE(k.dim() == 3 && k.size(1) == p.heads && k.size(2) == p.dim && k.stride(2) == 1 && v.sizes() == k.sizes() &&
-                        v.stride(2) == 1, "k and v must be [R, ", p.heads, ", ", p.dim, "] with unit last stride");
+  TORCH_CHECK_VALUE(k.dim() == 3 && k.size(1) == p.heads && k.size(2) == p.dim && k.stride(2) == 1 &&
+                        v.sizes() == k.sizes() && v.stride(2) == 1,
+                    "k and v must be [R, ", p.heads, ", ", p.dim, "] with unit last stride");
   TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type() && k.scalar_type() == kp.scalar_type(),
                    "k, v and the pages must share a dtype");
   const int64_t R = k.size(0);
@@ -130,7 +132,8 @@ PyObject* paged_append(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     const Tensor& q = tensor(arg[10], "q");
     on(q, index, "q");
     TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == R && q.size(2) == p.dim && q.stride(2) == 1 &&
-                          q.scalar_type() == k.scalar_type(), "q must be [", R, ", Hq, ", p.dim, "] of k's dtype with unit last stride");
+                          q.scalar_type() == k.scalar_type(),
+                      "q must be [", R, ", Hq, ", p.dim, "] of k's dtype with unit last stride");
     TORCH_CHECK_VALUE(a.inv_freq, "q without inv_freq: nothing rotates it");
     if (given(arg[11])) {
       out = tensor(arg[11], "q_out");
@@ -140,14 +143,16 @@ PyObject* paged_append(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     } else {
       out = at::empty(q.sizes(), q.options());
     }
-    a.q = q.data_ptr(), a.q_out = out.data_ptr(), a.q_ld = q.stride(0), a.q_sh = q.stride(1), a.Hq = small(q.size(1), "Hq");
+    a.q = q.data_ptr(), a.q_out = out.data_ptr(), a.q_ld = q.stride(0), a.q_sh = q.stride(1);
+    a.Hq = small(q.size(1), "Hq");
   } else {
     TORCH_CHECK_VALUE(!given(arg[11]), "q_out without q");
   }
   a.k = k.data_ptr(), a.v = v.data_ptr(), a.k_pages = kp.data_ptr(), a.v_pages = vp.data_ptr();
   a.k_ld = k.stride(0), a.k_sh = k.stride(1), a.v_ld = v.stride(0), a.v_sh = v.stride(1);
   a.page_stride = p.page_stride, a.head_stride = p.head_stride, a.num_pages = p.pages, a.table_ld = table.stride(0);
-  a.page_size = small(p.size, "page_size"), a.num_seqs = small(table.size(0), "table"), a.max_pages = small(table.size(1), "table");
+  a.page_size = small(p.size, "page_size"), a.num_seqs = small(table.size(0), "table");
+  a.max_pages = small(table.size(1), "table");
   a.R = small(R, "R"), a.Hkv = small(p.heads, "Hkv"), a.D = small(p.dim, "D"), a.dtype = dtype_code(k, "k");
   check(tread_paged_append(&a, stream_of(index)), "tread_paged_append");
   if (!out.defined()) Py_RETURN_NONE;
@@ -166,7 +171,8 @@ PyObject* paged_attn(PyObject*, PyObject* const* arg, Py_ssize_t count) {
   const Pools p = pools(kp, vp);
   on(vp, index, "v_pages"), on(q, index, "q");
   TORCH_CHECK_VALUE(q.dim() == 3 && q.size(2) == p.dim && q.stride(2) == 1 && (q.stride(1) == p.dim || q.size(1) <= 1) &&
-                        q.scalar_type() == kp.scalar_type(), "q must be [B, Hq, ", p.dim, "] of the pages' dtype with contiguous rows");
+                        q.scalar_type() == kp.scalar_type(),
+                    "q must be [B, Hq, ", p.dim, "] of the pages' dtype with contiguous rows");
   const int64_t B = q.size(0);
   tread_paged_attn_args a{};
   a.table = page_table(table, index);
@@ -193,7 +199,8 @@ PyObject* paged_attn(PyObject*, PyObject* const* arg, Py_ssize_t count) {
   // one workspace a call, from the allocator: calls of several streams, threads and graphs share none
   a.workspace_bytes = (int64_t)tread_paged_attn_workspace_bytes(a.Hq, a.Hkv, a.D);
   const Tensor ws = at::empty({a.workspace_bytes}, q.options().dtype(at::kByte));
-  a.workspace = ws.data_ptr(), a.q = q.data_ptr(), a.k_pages = kp.data_ptr(), a.v_pages = vp.data_ptr(), a.out = out.data_ptr();
+  a.workspace = ws.data_ptr(), a.q = q.data_ptr(), a.k_pages = kp.data_ptr(), a.v_pages = vp.data_ptr();
+  a.out = out.data_ptr();
   a.q_ld = q.stride(0), a.page_stride = p.page_stride, a.head_stride = p.head_stride, a.num_pages = p.pages;
   a.table_ld = table.stride(0), a.page_size = small(p.size, "page_size"), a.max_pages = small(table.size(1), "table");
   a.dtype = dtype_code(q, "q");
@@ -236,7 +243,8 @@ PyObject* adjust_logits(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     const Tensor& tokens = tensor(arg[1], "tokens");
     on(tokens, index, "tokens");
     TORCH_CHECK_VALUE(tokens.dim() == 2 && tokens.size(0) == B && tokens.scalar_type() == at::kLong &&
-                          (tokens.size(1) <= 1 || tokens.stride(1) == 1), "tokens must be int64 [", B, ", H] with unit column stride");
+                          (tokens.size(1) <= 1 || tokens.stride(1) == 1),
+                      "tokens must be int64 [", B, ", H] with unit column stride");
     a.tokens = static_cast<const int64_t*>(tokens.data_ptr()), a.tokens_ld = tokens.stride(0);
     a.max_tokens = small(tokens.size(1), "tokens");
     if (given(arg[2])) a.lens = vector<int64_t>(tensor(arg[2], "lens"), B, at::kLong, index, "lens");
@@ -254,8 +262,10 @@ PyObject* adjust_logits(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     const Tensor &ids = tensor(arg[7], "bias_ids"), &bias = tensor(arg[8], "bias");
     TORCH_CHECK_VALUE(ids.dim() >= 1, "bias_ids must have a last dimension");
     const int64_t n = ids.size(-1);
-    a.bias_ids_ld = by_row(ids, B, n, at::kLong, index, "bias_ids"), a.bias_ld = by_row(bias, B, n, at::kFloat, index, "bias");
-    a.bias_ids = static_cast<const int64_t*>(ids.data_ptr()), a.bias = static_cast<const float*>(bias.data_ptr());
+    a.bias_ids_ld = by_row(ids, B, n, at::kLong, index, "bias_ids");
+    a.bias_ld = by_row(bias, B, n, at::kFloat, index, "bias");
+    a.bias_ids = static_cast<const int64_t*>(ids.data_ptr());
+    a.bias = static_cast<const float*>(bias.data_ptr());
     a.num_bias = small(n, "bias_ids");
   }
   if (given(arg[9])) {
@@ -270,7 +280,8 @@ PyObject* adjust_logits(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     on(out, index, "out");
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == B && out.size(1) == V && (V <= 1 || out.stride(1) == 1),
                       "out must be [", B, ", ", V, "] with unit column stride");
-    TORCH_CHECK_VALUE(out.data_ptr() != x.data_ptr() || (out.scalar_type() == x.scalar_type() && out.stride(0) == x.stride(0)),
+    TORCH_CHECK_VALUE(out.data_ptr() != x.data_ptr() ||
+                          (out.scalar_type() == x.scalar_type() && out.stride(0) == x.stride(0)),
                       "out over logits must have their dtype and row stride");
   } else {
     out = at::empty({B, V}, x.options().dtype(at::kFloat));

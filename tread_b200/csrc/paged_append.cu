@@ -125,7 +125,9 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const __grid_
     for (int u = 0; u < kUnroll; ++u) {
       const int h = h0 + u * step, g = h - a.Hq;
       if (h >= heads) break;
-      T* to = g < 0 ? q_out + (long long)h * a.D : g < a.Hkv ? k_to + g * a.head_stride : v_to + (g - a.Hkv) * a.head_stride;
+      T* to = g < 0        ? q_out + (long long)h * a.D
+              : g < a.Hkv ? k_to + g * a.head_stride
+                          : v_to + (g - a.Hkv) * a.head_stride;
       if (dst < 0) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) x1[u].e[e] = x2[u].e[e] = Num<T>::from_f(0.f);
@@ -151,7 +153,7 @@ int launch(const AppendArgs& a, bool vec, cudaStream_t st) {
   // CTAs an SM, then heads. Rows for two an SM take 81 us instead of 79 at 16640 rows of 56 heads of 128, and
   // heads split until an SM has eight CTAs instead of four, 86.
   int tile_log2 = 0;
-  while ((2 << tile_log2) <= places && (2 << tile_log2) <= kMaxTile && ((long long)a.R >> (tile_log2 + 1)) >= 1184) ++tile_log2;
+  while ((2 << tile_log2) <= places && (2 << tile_log2) <= kMaxTile && (a.R >> (tile_log2 + 1)) >= 1184) ++tile_log2;
   const long long tiles = ((long long)a.R + (1 << tile_log2) - 1) >> tile_log2;
   const int lanes = places >> tile_log2;
   const long long passes = (a.Hq + 2LL * a.Hkv + lanes * kUnroll - 1) / (lanes * kUnroll);
@@ -192,9 +194,10 @@ extern "C" int tread_paged_append(const tread_paged_append_args* args, tread_str
   if (!a.rope_pos) a.rope_pos = a.pos;
   // 16-byte vectors where every head of every row starts on a 16-byte boundary, else single elements
   const int64_t ve = 16 / (int64_t)dtype_size(a.dtype);
-  const bool vec = (a.D / 2) % ve == 0 && (a.k_ld | a.k_sh | a.v_ld | a.v_sh | a.page_stride | a.head_stride) % ve == 0 &&
-                   (a.Hq == 0 || (a.q_ld | a.q_sh) % ve == 0) && aligned16(a.k) && aligned16(a.v) &&
-                   aligned16(a.k_pages) && aligned16(a.v_pages) && (a.Hq == 0 || (aligned16(a.q) && aligned16(a.q_out)));
+  const int64_t strides = a.k_ld | a.k_sh | a.v_ld | a.v_sh | a.page_stride | a.head_stride;
+  const bool vec = (a.D / 2) % ve == 0 && strides % ve == 0 && aligned16(a.k) && aligned16(a.v) &&
+                   aligned16(a.k_pages) && aligned16(a.v_pages) &&
+                   (a.Hq == 0 || ((a.q_ld | a.q_sh) % ve == 0 && aligned16(a.q) && aligned16(a.q_out)));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (a.dtype) {
     case TREAD_BF16: return launch<__nv_bfloat16>(a, vec, st);

@@ -498,11 +498,14 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
       is re-rotated by its offset).
     err: device error word; a row whose sequence, position or page is out of range appends nothing, gets
       a zero query and sets bit 0.
+    k, v and q must not overlap the pages. Any even D up to 256 and any page size.
     Returns the rotated queries [R, Hq, D] (q_out, which may be q itself), or None without q."""
     if stream is not None:
         with _on_stream(stream, k_pages):
-            return paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out, err)
-    return C.binding().paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out, err)
+            return paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out,
+                                err)
+    return C.binding().paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q,
+                                    q_out, err)
 
 
 def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=None, stream=None):
@@ -510,8 +513,11 @@ def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=No
     lens[b] tokens (int64 [B], the new token's own keys among them) in the pages table[b] (int32
     [B, pages]) of the pools [pages, Hkv, page_size, D], with GQA. Where no key
     has a score above -inf, or there is none (length 0), the output is zero.
-    err: device error word; a length that the table has no pages for gives a row of zeros and sets bit
-    1, and so does a page id outside the pool, whose keys count as masked. Returns out [B, Hq, D]."""
+    D in {64, 128, 256}, Hq / Hkv at most 16; q's rows, heads and pages on 16-byte boundaries; any page
+    size (multiples of 16 are read without a lookup per key). What slots behind a length hold does not
+    matter. err: device error word; a length that the table has no pages for gives a row of zeros and
+    sets bit 1; a page id outside the pool sets it too, and its keys count as masked.
+    Returns out [B, Hq, D] (out may be q itself)."""
     if stream is not None:
         with _on_stream(stream, k_pages):
             return paged_attn(q, k_pages, v_pages, table, lens, out, sm_scale, err)
@@ -532,11 +538,12 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
       of one token add up;
       -inf where the grammar does not allow it: bit v % 32 of allowed[..., v // 32] (int32 [B, W], or
       [W] for all rows, W = ceil(V / 32)) is 0.
-    Returns out: fp32 [B, V] by default; a given one may be of any supported dtype, or logits itself."""
+    V below 2^31 - 2^20, B at most 65535, N at most 2048. Returns out: fp32 [B, V] by default; a given one
+    may be of any supported dtype, or logits itself."""
     if stream is not None:
         with _on_stream(stream, logits):
-            return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, allowed,
-                                 out)
+            return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
+                                 allowed, out)
     return C.binding().adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
                                      allowed, out)
 

@@ -34,6 +34,7 @@ from fastapi import Depends, FastAPI, HTTPException, Request
 from pydantic import BaseModel, Field, StringConstraints
 
 from tread_b200 import kernels
+from tread_b200.paged import OutOfPages
 
 MAX_SEGMENT_CHARS = 200_000
 MAX_DOCUMENTS = 256
@@ -50,7 +51,7 @@ class CompletionRequest(BaseModel):
     max_tokens: int = Field(64, ge=1, le=2048)
     recompute_ratio: float = Field(0.2, ge=0.0, le=1.0)
     policy: str = Field("deviation", pattern="^(deviation|boundary|random)$")
-    repetition_penalty: float = Field(1.0, gt=0.0, le=100.0)
+    repetition_penalty: float = Field(1.0, ge=0.01, le=100.0)
     presence_penalty: float = Field(0.0, ge=-100.0, le=100.0)
     frequency_penalty: float = Field(0.0, ge=-100.0, le=100.0)
     logit_bias: dict[int, Annotated[float, Field(ge=-1e4, le=1e4)]] = Field(default_factory=dict, max_length=1024)
@@ -108,7 +109,8 @@ class _Adjust:
 
     def __call__(self, logits):
         """logits [vocab] -> adjusted fp32 [vocab]."""
-        return kernels.adjust_logits(logits[None], tokens=self.history[:, :self.n], prompt_lens=self.prompt, **self.kw)[0]
+        return kernels.adjust_logits(logits[None], tokens=self.history[:, :self.n], prompt_lens=self.prompt,
+                                     **self.kw)[0]
 
 
 def build_app(model, tok, engine, eos_ids, max_context=16384, api_key=None, max_queue=16, queue_timeout=30.0,
@@ -157,7 +159,7 @@ def build_app(model, tok, engine, eos_ids, max_context=16384, api_key=None, max_
             dev = logits.device
             try:
                 if decoder is not None:
-                    seq = decoder.admit(cache)
+                    seq = decoder.admit(cache, room=req.max_tokens)
                     cache = None
                 while nxt not in eos:
                     if len(out) >= req.max_tokens:
@@ -211,6 +213,8 @@ def build_app(model, tok, engine, eos_ids, max_context=16384, api_key=None, max_
                                     headers={"Retry-After": "5"})
             try:
                 return generate(req, ids)
+            except OutOfPages as e:  # a decoder that others use too
+                raise HTTPException(503, f"no room to decode: {e}", headers={"Retry-After": "5"}) from None
             finally:
                 gpu.release()
         finally:
