@@ -16,8 +16,7 @@
 // instructions cost it 3 us; finishing those tokens by themselves cost more, in scattered reads and writes of
 // lines that have left the caches: 26 us with their values found before the pass, 29 in place after it.
 // Reading the history again for every slice costs L2 reads only, and no counters in memory that a caller would
-// have to keep or clear. A warp that looks at 32 ids meets one of its slice nearly every time, so ids are only
-// sorted out there, and the slice's own are queued until 32 lanes have one each.
+// have to keep or clear.
 #include "common.cuh"
 
 namespace tread {
@@ -27,8 +26,7 @@ constexpr int kThreads = 256;
 constexpr int kMaxSlice = 18432;
 constexpr int kCtas = 4;         // CTAs of an SM
 constexpr int kVec = 8;          // consecutive logits of a thread
-constexpr int kQueue = 288;      // tokens of the slice that a warp gathers from the history
-constexpr int kQueuePrompt = 1 << 15;
+constexpr int kAhead = 8;        // ids of the history that a thread has in flight
 constexpr int kMaxBias = 2048;   // biases of a row: their values' room in shared memory
 
 using LogitsArgs = tread_adjust_logits_args;
@@ -82,7 +80,6 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   using C = Counter<W>;
   extern __shared__ __align__(16) unsigned char s_mem[];
   __shared__ int s_twice;   // some token of the slice has more than one bias
-  __shared__ uint16_t s_queue[kThreads / 32][kQueue];
   __shared__ float s_value[kMaxBias];
   W* count = reinterpret_cast<W*>(s_mem);  // of tokens first - kVec .. first + slice - 1
   const int b = blockIdx.y;
@@ -142,46 +139,29 @@ __global__ void __launch_bounds__(kThreads, kCtas)
         mine |= 1u << k;
     }
     if (a.tokens) {
-      const int lane = tid & 31;
       long long len = a.lens ? a.lens[b] : a.max_tokens;
       len = len < 0 ? 0 : len > a.max_tokens ? a.max_tokens : len;
       const long long prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
       const long long* ids = reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_ld;
-      uint16_t* queue = s_queue[tid >> 5];
-      int queued = 0;  // the same in all lanes
-      auto count_queued = [&]() {
-        __syncwarp();
-        for (int j = 0; j < queued; j += 32) {
-          if (j + lane >= queued) continue;
-          const int at = queue[j + lane] & (kQueuePrompt - 1);
-          if (queue[j + lane] & kQueuePrompt)
-            C::mark(count, at, C::kPrompt);
-          else
-            C::add(count, at);
-        }
-        __syncwarp();
-        queued = 0;
-      };
-      constexpr int kAhead = 8;
-      for (int i0 = tid - lane; i0 < (int)len; i0 += kThreads * kAhead) {
+      const unsigned room = end - begin;
+      for (int i0 = tid; i0 < (int)len; i0 += kThreads * kAhead) {
         long long v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-          const int i = i0 + lane + k * kThreads;
+          const int i = i0 + k * kThreads;
           v[k] = i < (int)len ? __ldg(ids + i) : -1;
         }
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-          const bool hit = v[k] >= begin && v[k] < end;
-          const unsigned who = __ballot_sync(0xffffffffu, hit);
-          if (hit)
-            queue[queued + __popc(who & ((1u << lane) - 1))] =
-                (uint16_t)(((int)v[k] - origin) | (i0 + lane + k * kThreads < prompt ? kQueuePrompt : 0));
-          queued += __popc(who);
+          const unsigned at = (unsigned)v[k] - (unsigned)begin;
+          if (at >= room || (v[k] >> 32) != 0) continue;
+          const int slot = (int)at + begin - origin;
+          if (i0 + k * kThreads < prompt)
+            C::mark(count, slot, C::kPrompt);
+          else
+            C::add(count, slot);
         }
-        if (queued > kQueue - 32 * kAhead) count_queued();
       }
-      count_queued();
     }
     __syncthreads();
     // the biased tokens, biases added up in the list's order
