@@ -273,7 +273,8 @@ int tread_rows_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
  *   inv_freq: DEVICE fp32 [D/2], or NULL: keys are copied (then Hq = 0). The angle is
  *             rope_pos * inv_freq in 64 bits; cos and sin times attn_scaling in fp32; rounded once.
  * A row whose sequence, position or page id is out of range appends nothing, gets a q_out row of zeros
- * and sets bit 0 of *err_flag (may be NULL). No two rows may name the same token; D even, at most 256.
+ * and sets bit 0 of *err_flag (may be NULL). No two rows may name the same token; k, v and q must not
+ * overlap the pools; D even, at most 256.
  * The arguments of this and the next two entry points come in a struct, read during the call only.
  */
 typedef struct {
@@ -293,8 +294,8 @@ int tread_paged_append(const tread_paged_append_args* args, tread_stream_t strea
  * Attention of one new token per sequence over its pages (the attention of tread/server.py:207-209's
  * decode forward): out[b, h] = softmax(sm_scale * q[b, h] . K[0..lens[b]-1, g]) V, g = h / (Hq / Hkv).
  *   q     : [B, Hq, D], rows q_ld apart; out: [B, Hq, D] contiguous
- *   table : device int32 [B, max_pages] at row stride table_ld; entries behind a sequence's last page
- *           are not read
+ *   table : device int32 [B, max_pages] at row stride table_ld (0: one row for all); entries behind a
+ *           sequence's last page are not read
  *   lens  : device int64 [B], keys of each sequence, the new token's own among them. Where no key has
  *           a score above -inf, or there is none, the output is zero
  * A length below 0 or above max_pages * page_size gives a row of zeros; keys in a page whose id is
@@ -323,10 +324,11 @@ int tread_paged_attn(const tread_paged_attn_args* args, tread_stream_t stream);
  * tread/server.py:203,210). Per row b, with n the count of token v in tokens[b, prompt_lens[b] : lens[b]]:
  *   x = logits[b, v];  if v is in tokens[b, 0 : lens[b]]: x = x > 0 ? x / repetition : x * repetition
  *   x -= frequency * n + presence * (n > 0);  x += the biases of v;  v not allowed: x = -inf
- * in fp32, rounded once to out_dtype.
- *   logits, out : [B, V] at row strides ld, ld_out; out may be logits itself (same type and stride)
- *   tokens      : device int64 [B, max_tokens] at row stride tokens_ld, or NULL; ids outside [0, V) count
- *                 for nothing. lens: device int64 [B] or NULL (max_tokens); prompt_lens: NULL is 0
+ * in fp32 (the quotient as a product with the reciprocal), rounded once to out_dtype.
+ *   logits, out : [B, V] at row strides ld, ld_out; out may be logits itself (same type and stride).
+ *                 B at most 65535, V at most 2^31 - 2^20
+ *   tokens      : device int64 [B, max_tokens] at row stride tokens_ld (0: one row for all), or NULL; ids
+ *                 outside [0, V) count for nothing. lens: device int64 [B] or NULL (max_tokens); prompt_lens: NULL is 0
  *   repetition, presence, frequency: device fp32 [B], or NULL: the value beside it for every row
  *                 (repetition above 0)
  *   bias_ids, bias: device int64 / fp32 [B, num_bias] at their row strides (0: one list for all rows);

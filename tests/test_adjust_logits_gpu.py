@@ -91,6 +91,21 @@ def test_numbers_and_shared_rows():
     _check(b, logits, **base, **per_row)
 
 
+def test_one_history_and_one_row_of_logits_for_all():
+    logits, kw = _case(4, 777, 60, BF, 16)
+    kw["tokens"], kw["lens"] = kw["tokens"][:1].expand(4, -1), kw["lens"][:1].repeat(4)
+    logits = logits[:1].expand(4, -1)
+    _check(kernels.adjust_logits(logits, **kw), logits, **kw)
+
+
+@pytest.mark.parametrize("rep", [1e-39, 1e-30, 1e30, 3e38])
+def test_repetition_far_from_one(rep):
+    """Reciprocals that overflow, lose digits or vanish."""
+    x = torch.tensor([[1e-3, -1e-3, 2e-39, -2e-39, 3.0, -3.0, 1e30, -1e30]], device=DEV)
+    kw = dict(tokens=torch.arange(8, device=DEV)[None], repetition=rep)
+    _check(kernels.adjust_logits(x, **kw), x, **kw)
+
+
 def test_padding_ids_and_lengths_out_of_range():
     logits, kw = _case(3, 500, 40, BF, 8)
     kw["tokens"][:, ::3] = -1

@@ -73,6 +73,19 @@ def test_append_rows(dtype, Hq, Hkv, D, page, counts, past):
     assert int(err) == 0
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_scaling(dtype):
+    """cos and sin times a factor: the rotation's bound times it, and two roundings more (2^-24 of the factor
+    each, inside the 2^-21)."""
+    q, k, v, kp, vp, table, pos, seq = _case([20], [700], 4, 2, 64, 16, dtype, 11)
+    inv, factor = inv_freq(64), 1.7
+    got = kernels.paged_append(k, v, kp, vp, table, pos, seq=seq, inv_freq=inv, attn_scaling=factor, q=q)
+    at, slot = table[0, pos // 16].long(), pos % 16
+    for a, x in ((got, q), (kp[at, :, slot], k)):
+        want = rotate64(x, pos, inv) * factor
+        assert bool(((a.double() - want).abs() <= factor * rotate_bound(x, want, dtype)).all())
+
+
 def test_append_without_seq_is_one_row_a_sequence():
     q, k, v, kp, vp, table, pos, seq = _case([1] * 6, [3, 0, 100, 64, 63, 5], 4, 2, 128, 64, BF, 2)
     kp2, vp2, inv = kp.clone(), vp.clone(), inv_freq(128)

@@ -167,6 +167,16 @@ def test_shared_pages_and_repeated_calls_give_the_same_bits():
         assert torch.equal(kernels.paged_attn(q, kp, vp, table, lens), got)
 
 
+def test_one_table_row_for_all_sequences():
+    """Several queries over the pages of one sequence (a table expanded by stride 0), at lengths of their own."""
+    q, kp, vp, table, _ = _case([1000], 28, 4, 128, 64, BF, 22)
+    g = _gen(23)
+    q = torch.randn(6, 28, 128, device=DEV, generator=g).to(BF)
+    lens = torch.tensor([1000, 1, 64, 999, 0, 500], device=DEV)
+    table = table.expand(6, -1)
+    _check(kernels.paged_attn(q, kp, vp, table, lens), q, kp, vp, table, lens)
+
+
 def test_output_over_the_queries():
     """out = q: every query is read before its row is written, in shares of one item and of several."""
     for lens in ([8000, 3], [60] * 100, [0, 5, 700]):

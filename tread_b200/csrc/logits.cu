@@ -44,10 +44,11 @@ struct Counter {
     const int shift = (i & 1) * 16;
     return atomicOr(reinterpret_cast<unsigned*>(c) + (i >> 1), what << shift) >> shift;
   }
-  static __device__ __forceinline__ unsigned add(W* c, int i) {
-    if constexpr (sizeof(W) == 4) return atomicAdd(reinterpret_cast<unsigned*>(c) + i, 1u);
-    const int shift = (i & 1) * 16;
-    return atomicAdd(reinterpret_cast<unsigned*>(c) + (i >> 1), 1u << shift) >> shift;
+  static __device__ __forceinline__ void add(W* c, int i) {
+    if constexpr (sizeof(W) == 4)
+      atomicAdd(reinterpret_cast<unsigned*>(c) + i, 1u);
+    else
+      atomicAdd(reinterpret_cast<unsigned*>(c) + (i >> 1), 1u << ((i & 1) * 16));
   }
 };
 
@@ -279,11 +280,15 @@ extern "C" int tread_adjust_logits(const tread_adjust_logits_args* args, tread_s
   TREAD_CHECK_ARG(a.B >= 0 && a.V >= 0, "adjust_logits: B < 0 or V < 0");
   if (a.B == 0 || a.V == 0) return TREAD_OK;
   TREAD_CHECK_ARG(a.logits && a.out, "adjust_logits: null pointer");
-  TREAD_CHECK_ARG(a.B <= 65535 && a.V <= INT32_MAX - (1 << 20), "adjust_logits: more than 65535 rows or 2^31 - 2^20 tokens");
+  TREAD_CHECK_ARG(a.B <= 65535 && a.V <= INT32_MAX - (1 << 20),
+                  "adjust_logits: more than 65535 rows or 2^31 - 2^20 tokens");
   TREAD_CHECK_ARG(dtype_size(a.dtype) != 0 && dtype_size(a.out_dtype) != 0, "adjust_logits: unknown dtype %d or %d",
                   a.dtype, a.out_dtype);
-  TREAD_CHECK_ARG(a.B == 1 || (a.ld >= a.V && a.ld_out >= a.V), "adjust_logits: row stride below the vocabulary");
-  TREAD_CHECK_ARG(a.max_tokens >= 0 && a.max_tokens <= (1 << 30) && (!a.tokens || a.B == 1 || a.tokens_ld >= a.max_tokens),
+  // an input's row stride may be 0: one row for all
+  TREAD_CHECK_ARG(a.B == 1 || ((a.ld == 0 || a.ld >= a.V) && a.ld_out >= a.V),
+                  "adjust_logits: row stride below the vocabulary");
+  TREAD_CHECK_ARG(a.max_tokens >= 0 && a.max_tokens <= (1 << 30) &&
+                      (!a.tokens || a.B == 1 || a.tokens_ld == 0 || a.tokens_ld >= a.max_tokens),
                   "adjust_logits: bad history");
   TREAD_CHECK_ARG(a.num_bias <= kMaxBias, "adjust_logits: more than %d biases", kMaxBias);
   TREAD_CHECK_ARG(a.num_bias >= 0 && (a.num_bias == 0 || (a.bias_ids && a.bias)), "adjust_logits: bad biases");

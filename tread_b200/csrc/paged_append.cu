@@ -188,7 +188,7 @@ extern "C" int tread_paged_append(const tread_paged_append_args* args, tread_str
                       (a.Hkv == 1 || a.head_stride >= (int64_t)a.page_size * a.D),
                   "paged_append: bad page geometry");
   TREAD_CHECK_ARG(a.num_seqs >= 0 && a.max_pages >= 0 && (a.table || a.num_seqs == 0 || a.max_pages == 0) &&
-                      (a.num_seqs <= 1 || a.table_ld >= a.max_pages),
+                      (a.num_seqs <= 1 || a.table_ld == 0 || a.table_ld >= a.max_pages),
                   "paged_append: bad page table");
   TREAD_CHECK_ARG(a.seq || a.R <= a.num_seqs, "paged_append: %d rows without seq, but %d sequences", a.R, a.num_seqs);
   if (!a.rope_pos) a.rope_pos = a.pos;

@@ -14,9 +14,9 @@
 // them, which are counted in. A CTA's share covers parts of one or more items (sequence, KV head). Its warps
 // take the units of the share in turn, each with a ring of units in flight in shared memory (cp.async, 16
 // bytes a lane, rows swizzled so that eight rows' same chunk lie in eight banks), its own running maximum
-// and sum, and its own accumulators. At an item's end the warps' states are joined in shared memory; an item that several
-// CTAs share leaves its states in the workspace, where a second kernel joins them in the order of the
-// shares (no atomics: the result does not depend on timing).
+// and sum, and its own accumulators. At an item's end the warps' states are joined in shared memory; an item
+// that several CTAs share leaves its states in the workspace, where a second kernel joins them in the order of
+// the shares (no atomics: the result does not depend on timing).
 //
 // 16-bit types run on mma.sync with keys as rows and the group's query heads as the 8 columns, so that a
 // group of 7 fills 7 of 8 columns (heads as rows would fill 7 of 16): S^T = K Q^T, O^T = V^T P^T, and the
@@ -789,7 +789,7 @@ extern "C" int tread_paged_attn(const tread_paged_attn_args* args, tread_stream_
                       (a.num_pages <= 1 || a.page_stride >= (int64_t)a.page_size * a.D) &&
                       (a.Hkv == 1 || a.head_stride >= (int64_t)a.page_size * a.D),
                   "paged_attn: bad page geometry");
-  TREAD_CHECK_ARG(a.max_pages >= 0 && (a.table || a.max_pages == 0) && (a.B <= 1 || a.table_ld >= a.max_pages),
+  TREAD_CHECK_ARG(a.max_pages >= 0 && (a.table || a.max_pages == 0) && (a.B <= 1 || a.table_ld == 0 || a.table_ld >= a.max_pages),
                   "paged_attn: bad page table");
   TREAD_CHECK_ARG((int64_t)a.max_pages * a.page_size <= INT32_MAX - kUnit,
                   "paged_attn: a sequence of 2^31 tokens or more");

@@ -120,6 +120,9 @@ class PagedDecoder:
         net = self.net = rows_of(model)
         if graphs and getattr(net, "world", 1) > 1:
             raise ValueError("graphs=True is not supported with tensor-parallel rows")
+        if net.D not in (64, 128, 256) or net.Hq > 16 * net.Hkv:
+            raise ValueError(f"paged attention takes heads of 64, 128 or 256 in groups of up to 16, not of {net.D} in "
+                             f"groups of {net.Hq // net.Hkv}")
         self.cache = PagedCache(net.L, net.Hkv, net.D, num_pages, page_size, max_seqs, max_len, net.dtype, net.device)
         self.inv_freq = torch.tensor(net.inv_freq, dtype=torch.float32, device=net.device)
         self.graphs = {} if graphs else None
