@@ -118,10 +118,11 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   // but for reciprocals that overflow or lose digits
   const float inv = 1.f / rep;
   const bool product = rep > 0x1p-100f && rep < 0x1p100f;
-  auto penalised = [&](float f, unsigned c) {  // c: not 0
-    f = f > 0.f ? (product ? f * inv : f / rep) : f * rep;
-    const unsigned n = c & C::kCount;
-    return n ? f - (freq * (float)n + pres) : f;
+  auto repeated = [&](float f) { return f > 0.f ? (product ? f * inv : f / rep) : f * rep; };
+  auto counted = [&](float f, unsigned c) { return f - (freq * (float)(c & C::kCount) + pres); };
+  auto penalised = [&](float f, unsigned c) {
+    if (c) f = repeated(f);
+    return c & C::kCount ? counted(f, c) : f;
   };
   unsigned mine = 0;  // biases whose token this thread marked first
   const int64_t* bias_ids = a.bias_ids + b * a.bias_ids_ld;
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
           if (bias_ids[j] == v) sum += bias[j];
       }
       const float f = Num<T>::to_f(row[v]);
-      s_value[i] = is_allowed(v) ? (c ? penalised(f, c) : f) + sum : -INFINITY;
+      s_value[i] = is_allowed(v) ? penalised(f, c) + sum : -INFINITY;
     }
     if (a.num_bias) __syncthreads();  // their logits are read before the pass writes them, where out is logits
   }
@@ -204,10 +205,23 @@ __global__ void __launch_bounds__(kThreads, kCtas)
           constexpr int E = 16 / sizeof(W);
           Vec16<W> c;
           c.raw = reinterpret_cast<const int4*>(count + (i + 1) * kVec)[j];
-          if (c.raw.x | c.raw.y | c.raw.z | c.raw.w) {
+          const unsigned any = c.raw.x | c.raw.y | c.raw.z | c.raw.w;
+          if (!any) continue;
+          if (product) {  // selects for all: a warp would go through every element's branch for one lane or another
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const float x = f[j * E + e];
+              f[j * E + e] = c.e[e] ? x * (x > 0.f ? inv : rep) : x;
+            }
+          } else {
+            for (int e = 0; e < E; ++e)
+              if (c.e[e]) f[j * E + e] = repeated(f[j * E + e]);
+          }
+          constexpr unsigned kCounts = sizeof(W) == 4 ? C::kCount : C::kCount * 0x10001u;
+          if (any & kCounts) {  // few are in the output
 #pragma unroll
             for (int e = 0; e < E; ++e)
-              if (c.e[e]) f[j * E + e] = penalised(f[j * E + e], c.e[e]);
+              if (c.e[e] & C::kCount) f[j * E + e] = counted(f[j * E + e], c.e[e]);
           }
         }
       }
@@ -235,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   auto single = [&](int v) {
     const float f = Num<T>::to_f(row[v]);
     const unsigned c = changes ? count[v - origin] : 0;
-    store(a.out, out_row + v, a.out_dtype, is_allowed(v) ? (c ? penalised(f, c) : f) : -INFINITY);
+    store(a.out, out_row + v, a.out_dtype, is_allowed(v) ? penalised(f, c) : -INFINITY);
   };
   if (tid < min(first, end) - begin) single(begin + tid);
   if (tid < end - first - vecs * kVec) single(first + vecs * kVec + tid);
