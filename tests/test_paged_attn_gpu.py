@@ -53,6 +53,14 @@ def test_lengths_around_every_edge(dtype, Hq, Hkv, D, page):
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_any_group(dtype, G, D):
+    c = _case([1, 0, 47, 300, 2111], 2 * G, 2, D, 16, dtype, G + D)
+    _check(kernels.paged_attn(*c), *c)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("page", [1, 3, 8, 20, 48, 128, 300])
 def test_any_page_size(dtype, page):
     c = _case([1, 7, 59, 100, 333], 14, 2, 64, page, dtype, page)
