@@ -10,11 +10,11 @@
 // first loads. While they fly it counts the row's whole history into counters of the slice in shared memory
 // (whole numbers: the order of the atomics does not matter), and computes the slice's few biased tokens, each by
 // the thread that marked it first. Then one pass reads, penalises, masks and stores every logit, and the biased
-// ones are stored again. At 64 rows of
-// 152064 with histories of up to 8768 that takes 22.5 us (2.8 TB/s; a casting copy of the same tensors takes 28),
-// the pass alone 13. Nearly every warp has one of the history's tokens among its 256, so the penalties'
-// instructions cost it 3 us; finishing those tokens by themselves cost more, in scattered reads and writes of
-// lines that have left the caches: 26 us with their values found before the pass, 29 in place after it.
+// ones are stored again. At 64 rows of 152064 with histories of up to 8768, a mask and 100 biases that takes
+// 19.2 us (3.2 TB/s; a casting copy of the same tensors takes 28), the pass alone 13.5. Nearly every warp has one of
+// the history's tokens among its 256, so the penalties are selects over a thread's vector rather than branches
+// (22.5 us). Finishing those tokens by themselves cost more, in scattered reads and writes of lines that have left
+// the caches: 26 us with their values found before the pass, 29 in place after it.
 // Reading the history again for every slice costs L2 reads only, and no counters in memory that a caller would
 // have to keep or clear.
 #include "common.cuh"
