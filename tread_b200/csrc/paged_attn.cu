@@ -27,7 +27,7 @@
 //
 // Measured, of 6.54 TB/s: 64 sequences of 2400-16640 tokens (28 / 4 heads of 128, bf16) 155 us, 6.2 TB/s; 18 of up
 // to 16640 (40 / 8 heads, fp16, pages of 16) 62 us, 5.9 TB/s; one of 8257 8.9 us, of which the two launches
-// take 3.3; 256 of 1-700 (14 / 2 heads of 64) 12.8 us. For small shares what counts is how little code runs: the
+// take 3.3; 256 of 1-700 (14 / 2 heads of 64) 12.5 us. For small shares what counts is how little code runs: the
 // fetch is in one place, and the line is summed in 32 bits.
 #include <type_traits>
 
@@ -125,16 +125,20 @@ __device__ __forceinline__ int place_of(int h, int d) {
   return h * D + (d ^ (((h >> 1) & 3) << 3));
 }
 
-// Shared memory and launch shape of one instance. Two CTAs per SM where their rings fit beside each
-// other, so that one joins while the other streams; about 190 KB of units in flight per SM either way.
+// Shared memory and launch shape of one instance. Two CTAs per SM where their rings fit beside each other, so that
+// one joins while the other streams; 130 to 190 KB of units in flight per SM. For 16 heads of 128 on one KV head
+// (16-bit) 60 sequences of up to 4000 tokens take 19.3 us, 23.1 with one CTA and three times the stages, 200 of
+// 5-20 10.9 and 12.9; one of 8000 10.1 and 9.3. Longer keys fit twice with half the warps only. That pays where a
+// unit is little work, with one head (fp32, 8/8 heads of 128, 200 of 5-20: 30 -> 19 us, long ones alike), and is
+// slower at most lengths elsewhere (16/2 heads of 256, bf16, 150 of 20-500: 23.7 -> 27.0 us).
 template <typename T, int D, int GP>
 struct Shape {
   static constexpr int kRow = D * sizeof(T);               // bytes of one key
   static constexpr int kUnitBytes = 2 * kUnit * kRow;      // keys, then values
-  static constexpr int kWarps = kUnitBytes > 16384 ? 2 : 4;
+  static constexpr int kWarps = kUnitBytes > (GP == 1 ? 8192 : 16384) ? 2 : 4;
   static constexpr int kJoin = kWarps * GP * D * 4;        // the warps' accumulators at an item's end
   static constexpr int kQ = sizeof(T) == 4 ? GP * D * 4 + kWarps * kUnit * GP * 4 : 0;  // fp32: queries and weights
-  static constexpr int kCtas = kUnitBytes <= 8192 && kJoin <= 16384 ? 2 : 1;
+  static constexpr int kCtas = kWarps * kUnitBytes <= 32768 ? 2 : 1;
   static constexpr int kRoom = (kCtas == 2 ? 112 : 224) * 1024 - kJoin - kQ;
   static constexpr int kFit = kRoom / (kWarps * kUnitBytes);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
@@ -292,7 +296,7 @@ struct FmaState {
     float s[GP];
 #pragma unroll
     for (int h = 0; h < GP; ++h) s[h] = 0.f;
-#pragma unroll 4
+#pragma unroll (GP < 8 ? 8 : 4)
     for (int i = 0; i < D / 8; ++i) {
       const int c = half * (D / 8) + i;
       float4 k;
@@ -340,7 +344,7 @@ struct FmaState {
       }
     }
     __syncwarp();
-#pragma unroll 4
+#pragma unroll (GP < 8 ? 8 : 4)
     for (int t = 0; t < kUnit; ++t) {
       float v[kPer];
       if constexpr (kPer == 2) {
@@ -417,8 +421,10 @@ struct Place {
   }
 };
 
+// The CTAs of an SM stand in the bounds even where they are one: without them the compiler saves registers for
+// more, and fp32 takes up to twice as long (16/1 heads of 128, 60 sequences of up to 4000: 118 us, 59 with).
 template <typename T, int D, int GP, bool WHOLE>  // WHOLE: a unit never crosses a page (page_size % 16 == 0)
-__global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32)
+__global__ void __launch_bounds__(Shape<T, D, GP>::kWarps * 32, Shape<T, D, GP>::kCtas)
     paged_attn_kernel(const __grid_constant__ DecodeArgs a) {
   using S = Shape<T, D, GP>;
   constexpr int W = S::kWarps, kThreads = W * 32, kStages = S::kStages;
@@ -762,7 +768,8 @@ int launch_width(int D, const DecodeArgs& a, int sms, cudaStream_t st) {
 template <typename T>
 int dispatch(int D, const DecodeArgs& a, int sms, cudaStream_t st) {
   // On FMAs a head that is not there costs as much as others, so fp32 has narrower instances too. 32 sequences of
-  // 2000 tokens, D = 128: 16/8 heads 145 us with eight wide, 107 us with four; 8/8 heads 145 and 87 us with one.
+  // 2000 tokens, D = 128, when these were made: 16/8 heads 145 us with eight wide, 107 us with four; 8/8 heads 145
+  // and 87 us with one.
   // (A column of the tensor cores' tiles costs nothing; eight is their width.)
   if constexpr (sizeof(T) == 4) {
     if (a.G == 1) return launch_width<T, 1>(D, a, sms, st);
