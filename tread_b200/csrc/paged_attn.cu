@@ -205,8 +205,9 @@ struct MmaState {
         if (!live1) x[2] = x[3] = -INFINITY;
       }
       float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
-      // the maximum moves only when a score leaves it behind by more than kSlack: rarely
-      if (__any_sync(0xffffffffu, top[0] > m[nt][0] + kSlack || top[1] > m[nt][1] + kSlack)) {
+      // the maximum moves only when a score leaves it behind by more than kSlack: rarely. The difference, since a
+      // sum with a large maximum would be rounded; -inf and NaN compare false.
+      if (__any_sync(0xffffffffu, top[0] - m[nt][0] > kSlack || top[1] - m[nt][1] > kSlack)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -319,7 +320,7 @@ struct FmaState {
     for (int h = 0; h < GP; ++h) {
       s[h] = (s[h] + __shfl_xor_sync(0xffffffffu, s[h], 16)) * a.scale_log2;
       if (!on) s[h] = -INFINITY;
-      moved |= s[h] > m[h] + kSlack;
+      moved |= s[h] - m[h] > kSlack;
     }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
