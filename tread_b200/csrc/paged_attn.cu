@@ -21,8 +21,9 @@
 // 16-bit types run on mma.sync with keys as rows and the group's query heads as the 8 columns, so that a
 // group of 7 fills 7 of 8 columns (heads as rows would fill 7 of 16): S^T = K Q^T, O^T = V^T P^T, and the
 // heads of S^T's, P^T's and O^T's columns stay in the same lanes. P meets V as the sum of two numbers of the
-// type, its rounding and what that left out: the weights keep 16 bits or more, and the output's own rounding
-// is all that is lost (rounded once, the weights add as much error again); 1 % of the time.
+// type, its rounding and what that left out: the weights keep 16 bits or more (in fp16 down to 2^-22 of the
+// largest weight, see Range), and the output's own rounding is nearly all that is lost (rounded once, the weights
+// add as much error again); 1 % of the time.
 // fp32 runs on FMAs.
 //
 // Measured, of 6.54 TB/s: 64 sequences of 2400-16640 tokens (28 / 4 heads of 128, bf16) 155 us, 6.2 TB/s; 18 of up
@@ -41,7 +42,17 @@ constexpr int kMaxCtas = 384;  // shares at most
 constexpr int kItemCost = 8;   // units that an item's fixed cost amounts to
 constexpr int kMinShare = 4;   // a unit for every warp: more parts cost more to join
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;  // the running maximum may lag by 2^8: weights stay far inside fp16's range
+
+// The running maximum may lag behind the scores by kSlack (a weight is at most 2^kSlack), and 16-bit weights are
+// formed 2^kRaise times too large: sums and accumulators carry the same factor, the quotient drops it. bf16 reaches
+// as far down as fp32. fp16 ends at 2^-24 and 2^16: raised as far as it goes, a weight's second part is off by at
+// most 2^-25-13 = 2^-38 of the largest weight, so that keys 2^-27 below one key (an attention sink whose value is
+// near zero) keep the 11 bits of the output; unraised, they were lost from 2^-14 on.
+template <typename T>
+struct Range {
+  static constexpr float kSlack = std::is_same<T, __half>::value ? 2.f : 8.f;
+  static constexpr float kRaise = std::is_same<T, __half>::value ? 8192.f : 1.f;
+};
 
 struct DecodeArgs : tread_paged_attn_args {
   int G;
@@ -207,6 +218,7 @@ struct MmaState {
       float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
       // the maximum moves only when a score leaves it behind by more than kSlack: rarely. The difference, since a
       // sum with a large maximum would be rounded; -inf and NaN compare false.
+      constexpr float kSlack = Range<T>::kSlack;
       if (__any_sync(0xffffffffu, top[0] - m[nt][0] > kSlack || top[1] - m[nt][1] > kSlack)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -221,7 +233,7 @@ struct MmaState {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = weight(x[i], m[nt][i & 1]);
+      for (int i = 0; i < 4; ++i) x[i] = weight(x[i], m[nt][i & 1]) * Range<T>::kRaise;
       l[nt][0] += x[0] + x[2];
       l[nt][1] += x[1] + x[3];
       p[nt][0] = transpose8x8(pack2<T>(x[0], x[1]));
@@ -320,7 +332,7 @@ struct FmaState {
     for (int h = 0; h < GP; ++h) {
       s[h] = (s[h] + __shfl_xor_sync(0xffffffffu, s[h], 16)) * a.scale_log2;
       if (!on) s[h] = -INFINITY;
-      moved |= s[h] - m[h] > kSlack;
+      moved |= s[h] - m[h] > Range<float>::kSlack;
     }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
