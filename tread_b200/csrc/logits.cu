@@ -272,7 +272,10 @@ int launch(const LogitsArgs& a, cudaStream_t st) {
   const int slice = (((a.V + slices - 1) / slices) + 63) / 64 * 64;  // whole vectors of counters
   const int smem = (slice + kVec) * (int)sizeof(W);
   auto kern = adjust_logits_kernel<T, W, VECS>;
-  if (smem > 24 * 1024) TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the largest slice's, not this call's: another host thread may be between here and its launch
+  if (smem > 24 * 1024)
+    TREAD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (kMaxSlice + kVec) * (int)sizeof(W)));
   kern<<<dim3(slices, a.B), kThreads, smem, st>>>(a, slice);
   TREAD_CHECK_LAUNCH("adjust_logits_kernel");
   return TREAD_OK;
