@@ -328,7 +328,8 @@ int tread_paged_attn(const tread_paged_attn_args* args, tread_stream_t stream);
  *   logits, out : [B, V] at row strides ld, ld_out; out may be logits itself (same type and stride).
  *                 B at most 65535, V at most 2^31 - 2^20
  *   tokens      : device int64 [B, max_tokens] at row stride tokens_ld (0: one row for all), or NULL; ids
- *                 outside [0, V) count for nothing. lens: device int64 [B] or NULL (max_tokens); prompt_lens: NULL is 0
+ *                 outside [0, V) count for nothing; max_tokens below 2^30
+ *   lens, prompt_lens: device int64 [B], or NULL: max_tokens and 0
  *   repetition, presence, frequency: device fp32 [B], or NULL: the value beside it for every row
  *                 (repetition above 0)
  *   bias_ids, bias: device int64 / fp32 [B, num_bias] at their row strides (0: one list for all rows);

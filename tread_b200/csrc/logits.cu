@@ -304,7 +304,8 @@ extern "C" int tread_adjust_logits(const tread_adjust_logits_args* args, tread_s
   // an input's row stride may be 0: one row for all
   TREAD_CHECK_ARG(a.B == 1 || ((a.ld == 0 || a.ld >= a.V) && a.ld_out >= a.V),
                   "adjust_logits: row stride below the vocabulary");
-  TREAD_CHECK_ARG(a.max_tokens >= 0 && a.max_tokens <= (1 << 30) &&
+  // a count fits below a 32-bit counter's two marks
+  TREAD_CHECK_ARG(a.max_tokens >= 0 && a.max_tokens < (1 << 30) &&
                       (!a.tokens || a.B == 1 || a.tokens_ld == 0 || a.tokens_ld >= a.max_tokens),
                   "adjust_logits: bad history");
   TREAD_CHECK_ARG(a.num_bias <= kMaxBias, "adjust_logits: more than %d biases", kMaxBias);

@@ -538,8 +538,8 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
       of one token add up;
       -inf where the grammar does not allow it: bit v % 32 of allowed[..., v // 32] (int32 [B, W], or
       [W] for all rows, W = ceil(V / 32)) is 0.
-    V below 2^31 - 2^20, B at most 65535, N at most 2048. Returns out: fp32 [B, V] by default; a given one
-    may be of any supported dtype, or logits itself."""
+    V at most 2^31 - 2^20, H below 2^30, B at most 65535, N at most 2048. Returns out: fp32 [B, V] by default; a
+    given one may be of any supported dtype, or logits itself."""
     if stream is not None:
         with _on_stream(stream, logits):
             return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
