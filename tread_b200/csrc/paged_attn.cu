@@ -22,7 +22,7 @@
 // group of 7 fills 7 of 8 columns (heads as rows would fill 7 of 16): S^T = K Q^T, O^T = V^T P^T, and the
 // heads of S^T's, P^T's and O^T's columns stay in the same lanes. P meets V as the sum of two numbers of the
 // type, its rounding and what that left out: the weights keep 16 bits or more (in fp16 down to 2^-22 of the
-// largest weight, see Range), and the output's own rounding is nearly all that is lost (rounded once, the weights
+// largest weight, see kRaise), and the output's own rounding is nearly all that is lost (rounded once, the weights
 // add as much error again); 1 % of the time.
 // fp32 runs on FMAs.
 //
@@ -49,10 +49,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // most 2^-25-13 = 2^-38 of the largest weight, so that keys 2^-27 below one key (an attention sink whose value is
 // near zero) keep the 11 bits of the output; unraised, they were lost from 2^-14 on.
 template <typename T>
-struct Range {
-  static constexpr float kSlack = std::is_same<T, __half>::value ? 2.f : 8.f;
-  static constexpr float kRaise = std::is_same<T, __half>::value ? 8192.f : 1.f;
-};
+constexpr float kSlack = std::is_same<T, __half>::value ? 2.f : 8.f;
+template <typename T>
+constexpr float kRaise = std::is_same<T, __half>::value ? 8192.f : 1.f;
 
 struct DecodeArgs : tread_paged_attn_args {
   int G;
@@ -218,8 +217,7 @@ struct MmaState {
       float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
       // the maximum moves only when a score leaves it behind by more than kSlack: rarely. The difference, since a
       // sum with a large maximum would be rounded; -inf and NaN compare false.
-      constexpr float kSlack = Range<T>::kSlack;
-      if (__any_sync(0xffffffffu, top[0] - m[nt][0] > kSlack || top[1] - m[nt][1] > kSlack)) {
+      if (__any_sync(0xffffffffu, top[0] - m[nt][0] > kSlack<T> || top[1] - m[nt][1] > kSlack<T>)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -233,7 +231,7 @@ struct MmaState {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = weight(x[i], m[nt][i & 1]) * Range<T>::kRaise;
+      for (int i = 0; i < 4; ++i) x[i] = weight(x[i], m[nt][i & 1]) * kRaise<T>;
       l[nt][0] += x[0] + x[2];
       l[nt][1] += x[1] + x[3];
       p[nt][0] = transpose8x8(pack2<T>(x[0], x[1]));
@@ -332,7 +330,7 @@ struct FmaState {
     for (int h = 0; h < GP; ++h) {
       s[h] = (s[h] + __shfl_xor_sync(0xffffffffu, s[h], 16)) * a.scale_log2;
       if (!on) s[h] = -INFINITY;
-      moved |= s[h] - m[h] > Range<float>::kSlack;
+      moved |= s[h] - m[h] > kSlack<float>;
     }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
