@@ -192,6 +192,11 @@ extern "C" int tread_paged_append(const tread_paged_append_args* args, tread_str
                   "paged_append: bad page table");
   TREAD_CHECK_ARG(a.seq || a.R <= a.num_seqs, "paged_append: %d rows without seq, but %d sequences", a.R, a.num_seqs);
   if (!a.rope_pos) a.rope_pos = a.pos;
+  // the stride of a dimension of one is any number
+  if (a.R == 1) a.k_ld = a.v_ld = a.q_ld = 0;
+  if (a.Hq == 1) a.q_sh = 0;
+  if (a.Hkv == 1) a.k_sh = a.v_sh = a.head_stride = 0;
+  if (a.num_pages <= 1) a.page_stride = 0;
   // 16-byte vectors where every head of every row starts on a 16-byte boundary, else single elements
   const int64_t ve = 16 / (int64_t)dtype_size(a.dtype);
   const int64_t strides = a.k_ld | a.k_sh | a.v_ld | a.v_sh | a.page_stride | a.head_stride;

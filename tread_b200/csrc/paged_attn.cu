@@ -824,6 +824,10 @@ extern "C" int tread_paged_attn(const tread_paged_attn_args* args, tread_stream_
                   "paged_attn: a sequence of 2^31 tokens or more");
   TREAD_CHECK_ARG(((int64_t)a.max_pages * a.page_size / kUnit + 1 + kItemCost) * a.Hkv <= (1 << 30) / a.B,
                   "paged_attn: a table of more than 2^34 tokens, counted by KV head");
+  // the stride of a dimension of one is any number
+  if (a.B == 1) a.q_ld = 0;
+  if (a.num_pages <= 1) a.page_stride = 0;
+  if (a.Hkv == 1) a.head_stride = 0;
   TREAD_CHECK_ARG(aligned16(a.q) && aligned16(a.k_pages) && aligned16(a.v_pages) && aligned16(a.out) &&
                       ((a.q_ld | a.page_stride | a.head_stride) * es) % 16 == 0,
                   "paged_attn: q, out and pages must lie on 16-byte boundaries");
