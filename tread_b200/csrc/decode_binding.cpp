@@ -7,7 +7,10 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
+#include <utility>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -91,6 +94,44 @@ const int32_t* page_table(const Tensor& t, c10::DeviceIndex index) {
   return static_cast<const int32_t*>(t.data_ptr());
 }
 
+// The runs of consecutive bytes of a tensor with unit last stride, in order of address.
+std::vector<std::pair<uintptr_t, uintptr_t>> runs(const Tensor& t) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> r;
+  const int64_t es = t.element_size(), width = t.size(-1) * es, d = t.dim();
+  const int64_t n0 = t.size(0), n1 = d == 3 ? t.size(1) : 1, s0 = t.stride(0) * es, s1 = d == 3 ? t.stride(1) * es : 0;
+  for (int64_t i = 0; i < n0; ++i)
+    for (int64_t j = 0; j < n1; ++j) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr()) + i * s0 + j * s1;
+      r.emplace_back(at, at + width);
+    }
+  std::sort(r.begin(), r.end());
+  return r;
+}
+
+// An output may be an input itself (each element is read before it is written, by the thread that writes it) where
+// `itself` says so, or lie apart from it; its elements over others of the input would be a race.
+void apart(const Tensor& out, const Tensor& in, bool itself, const char* out_name, const char* in_name) {
+  if (out.numel() == 0 || in.numel() == 0) return;
+  auto end = [](const Tensor& t) {
+    int64_t last = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) + last * t.element_size();
+  };
+  const uintptr_t a = reinterpret_cast<uintptr_t>(out.data_ptr()), b = reinterpret_cast<uintptr_t>(in.data_ptr());
+  if (a >= end(in) || b >= end(out)) return;
+  if (itself && a == b && out.scalar_type() == in.scalar_type() && out.sizes() == in.sizes()) {
+    bool same = true;
+    for (int64_t i = 0; i < out.dim(); ++i) same &= out.size(i) == 1 || out.stride(i) == in.stride(i);
+    if (same) return;
+  }
+  const auto x = runs(out), y = runs(in);  // columns of one buffer may lie between each other
+  for (size_t i = 0, j = 0; i < x.size() && j < y.size();) {
+    TORCH_CHECK_VALUE(x[i].second <= y[j].first || y[j].second <= x[i].first, out_name, " overlaps ", in_name,
+                      " in memory", itself ? ", but is not the same elements" : "");
+    x[i].second <= y[j].first ? ++i : ++j;
+  }
+}
+
 void check(int rc, const char* what) {
   TORCH_CHECK(rc == TREAD_OK, what, " failed (status ", rc, "): ", tread_last_error());
 }
@@ -140,6 +181,7 @@ PyObject* paged_append(PyObject*, PyObject* const* arg, Py_ssize_t count) {
       on(out, index, "q_out");
       TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.is_contiguous(),
                         "q_out must be a contiguous tensor of q's shape and dtype");
+      apart(out, q, true, "q_out", "q"), apart(out, k, false, "q_out", "k"), apart(out, v, false, "q_out", "v");
     } else {
       out = at::empty(q.sizes(), q.options());
     }
@@ -192,6 +234,7 @@ PyObject* paged_attn(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     on(out, index, "out");
     TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.is_contiguous(),
                       "out must be a contiguous tensor of q's shape and dtype");
+    apart(out, q, true, "out", "q");
   } else {
     out = at::empty(q.sizes(), q.options());
   }
@@ -280,9 +323,7 @@ PyObject* adjust_logits(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     on(out, index, "out");
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == B && out.size(1) == V && (V <= 1 || out.stride(1) == 1),
                       "out must be [", B, ", ", V, "] with unit column stride");
-    TORCH_CHECK_VALUE(out.data_ptr() != x.data_ptr() ||
-                          (out.scalar_type() == x.scalar_type() && out.stride(0) == x.stride(0)),
-                      "out over logits must have their dtype and row stride");
+    apart(out, x, true, "out", "logits");
   } else {
     out = at::empty({B, V}, x.options().dtype(at::kFloat));
   }

@@ -499,7 +499,8 @@ def paged_append(k, v, k_pages, v_pages, table, pos, seq=None, inv_freq=None, ro
     err: device error word; a row whose sequence, position or page is out of range appends nothing, gets
       a zero query and sets bit 0.
     k, v and q must not overlap the pages. Any even D up to 256 and any page size.
-    Returns the rotated queries [R, Hq, D] (q_out, which may be q itself), or None without q."""
+    Returns the rotated queries [R, Hq, D] (q_out, which may be q itself and else overlaps neither q, k nor v), or
+    None without q."""
     if stream is not None:
         with _on_stream(stream, k_pages):
             return paged_append(k, v, k_pages, v_pages, table, pos, seq, inv_freq, rope_pos, attn_scaling, q, q_out,
@@ -517,7 +518,7 @@ def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=No
     size (multiples of 16 are read without a lookup per key). What slots behind a length hold does not
     matter. err: device error word; a length that the table has no pages for gives a row of zeros and
     sets bit 1; a page id outside the pool sets it too, and its keys count as masked.
-    Returns out [B, Hq, D] (out may be q itself)."""
+    Returns out [B, Hq, D] (out may be q itself, and else does not overlap it)."""
     if stream is not None:
         with _on_stream(stream, k_pages):
             return paged_attn(q, k_pages, v_pages, table, lens, out, sm_scale, err)
@@ -539,7 +540,7 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=1
       -inf where the grammar does not allow it: bit v % 32 of allowed[..., v // 32] (int32 [B, W], or
       [W] for all rows, W = ceil(V / 32)) is 0.
     V at most 2^31 - 2^20, H below 2^30, B at most 65535, N at most 2048. Returns out: fp32 [B, V] by default; a
-    given one may be of any supported dtype, or logits itself."""
+    given one may be of any supported dtype; it may be logits itself, and else does not overlap them."""
     if stream is not None:
         with _on_stream(stream, logits):
             return adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
