@@ -141,7 +141,12 @@ class PagedDecoder:
         values = [layer.values for layer in cache.layers]
         if len(keys) != self.net.L:
             raise ValueError(f"admit: a cache of {len(keys)} layers, the model has {self.net.L}")
-        T = keys[0].shape[2]
+        T = keys[0].shape[2] if keys[0].dim() == 4 else 0
+        want = (1, self.net.Hkv, T, self.net.D)
+        for t in keys + values:
+            if t.shape != want:
+                raise ValueError(f"admit: layers must be [1, {self.net.Hkv}, T, {self.net.D}] of one length, got "
+                                 f"{list(t.shape)}")
         pc = self.cache
         seq = pc.new(T + room)
         try:
