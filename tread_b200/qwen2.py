@@ -167,6 +167,7 @@ class Qwen2Rows:
         return (torch.zeros(shape, dtype=self.dtype, device=self.device),
                 torch.zeros(shape, dtype=self.dtype, device=self.device))
 
+    @torch.inference_mode()  # the words may have been made in it, and are then cleared in it only
     def check_errors(self):
         """Raise if a kernel flagged an out-of-range row position: the row kernels' error word and
         the selector's sticky flag, read with one device sync."""

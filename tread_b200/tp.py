@@ -217,6 +217,7 @@ class TPQwen2Rows(Qwen2Rows):
         allnorms = self._timed("head_norms_allgather", lambda: gather_head_norms(norms, self.group))
         return kernels.select_head_norms(allnorms, cand_pos, budget)
 
+    @torch.inference_mode()  # the words may have been made in it, and are then cleared in it only
     def check_errors(self):
         """Raise on every rank if a kernel on any rank flagged an error (row kernels' error word
         or the selector's out-of-range flag), with one all-reduce."""
