@@ -29,7 +29,8 @@ class OutOfPages(RuntimeError):
 class PagedCache:
     """Pools of pages [num_pages, L, Hkv, page_size, D] for K and V, and the page tables of up to
     `max_seqs` sequences of up to `max_len` tokens. The bookkeeping is the host's; the tables are on the
-    device, int32 [max_seqs, pages of max_len], entries of pages that a sequence does not hold -1."""
+    device, int32 [max_seqs, pages of max_len], entries of pages that a sequence does not hold -1. Made inside
+    inference mode or outside of it, it is used in either."""
 
     def __init__(self, L, Hkv, D, num_pages, page_size=64, max_seqs=64, max_len=32768, dtype=torch.bfloat16,
                  device="cuda"):
@@ -56,6 +57,7 @@ class PagedCache:
         """The pools of layer l, views [num_pages, Hkv, page_size, D]."""
         return self.K[:, l], self.V[:, l]
 
+    @torch.inference_mode()
     def new(self, tokens=0):
         """A new sequence with room for `tokens` tokens; it holds none yet."""
         if not self._free_seqs:
@@ -69,6 +71,7 @@ class PagedCache:
             raise
         return seq
 
+    @torch.inference_mode()
     def reserve(self, seq, tokens):
         """Give `seq` pages for `tokens` tokens in all (nothing changes if that fails)."""
         pages = self._pages[seq]
@@ -87,6 +90,7 @@ class PagedCache:
         else:
             self.table[seq, at:at + need] = torch.tensor(new, dtype=torch.int32).to(self.table.device)
 
+    @torch.inference_mode()
     def release(self, seq):
         """Give back the sequence and its pages."""
         if seq not in self.lens:
