@@ -43,3 +43,21 @@ def test_admit_refuses_a_batch_of_one_layer():
     with pytest.raises(ValueError, match="admit: layers"):
         dec.admit(_cache([((2, 2, 5, 64), (2, 2, 5, 64))]))
     assert _unchanged(dec)
+
+
+@pytest.mark.parametrize("tokens", [[-1], [50], torch.tensor([50]), torch.tensor([-1], dtype=torch.int32), [1.5],
+                                    torch.tensor([1.0]), torch.tensor([[1]]), [[1]], torch.tensor([True]), [1, 2], []])
+def test_step_refuses_tokens(tokens):
+    """Outside the vocabulary, not whole numbers, not one a sequence."""
+    dec = _decoder()
+    seq = dec.cache.new(0)
+    with pytest.raises(ValueError, match="step: "):
+        dec.step([seq], tokens)
+    assert dec.cache.lens == {seq: 0} and dec.cache.free_pages == 10
+
+
+def test_token_ids_of_any_whole_type():
+    dec = _decoder()
+    for tokens in ([0, 49], torch.tensor([0, 49]), torch.tensor([0, 49], dtype=torch.int16), (0, 49)):
+        ids = dec._ids(tokens)
+        assert ids.dtype == torch.int64 and ids.tolist() == [0, 49]

@@ -191,12 +191,32 @@ class PagedDecoder:
             h = net.layer_tail(l, h, o.view(B, nq))
         return net.logits(h)
 
+    def _ids(self, tokens):
+        """Token ids [B] as an int64 device tensor, all inside the vocabulary: an embedding lookup outside it is a
+        device-side assertion, after which the process has no GPU."""
+        net = self.net
+        t = torch.as_tensor(tokens)
+        if t.dim() != 1 or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+            raise ValueError(f"step: tokens must be whole numbers, one a sequence, got {t.dtype} {list(t.shape)}")
+        vocab = net.embed.shape[0]
+        if t.is_cuda:  # not read back: the step runs with the nearest id, and check_errors() raises
+            t = t.to(net.device, torch.int64)
+            ids = t.clamp(0, vocab - 1)
+            net.err[:1].bitwise_or_((ids != t).any().to(torch.int32))
+            return ids
+        t = t.to(torch.int64)
+        if int(t.min()) < 0 or int(t.max()) >= vocab:
+            raise ValueError(f"step: token ids from {int(t.min())} to {int(t.max())}, the vocabulary has {vocab}")
+        return t.to(net.device)
+
     @torch.inference_mode()
     def step(self, seqs, tokens):
         """Append tokens[i] to sequence seqs[i] and return the logits of what follows, [len(seqs), vocab].
-        seqs: distinct sequences; tokens: their ids, a list or an int64 tensor. Where a sequence's pages do
-        not suffice, nothing happens and OutOfPages (or ValueError past max_len) is raised. With graphs
-        the result is the graph's own buffer, valid until the next step of that batch size."""
+        seqs: distinct sequences; tokens: their ids, a list or a tensor of whole numbers [len(seqs)]. Ids outside
+        the vocabulary are refused; those of a device tensor, which is not read back, are replaced by the nearest
+        one, and net.check_errors() raises. Where a sequence's pages do not suffice, nothing happens and
+        OutOfPages (or ValueError past max_len) is raised. With graphs the result is the graph's own buffer,
+        valid until the next step (a graph serves all batch sizes up to its power of two)."""
         pc, dev = self.cache, self.net.device
         B = len(seqs)
         if B == 0 or len(set(seqs)) != B or not all(s in pc.lens for s in seqs):
@@ -209,11 +229,11 @@ class PagedDecoder:
         short = sum(max(0, pc.pages_of(n) - len(pc._pages[s])) for s, n in zip(seqs, need))
         if short > pc.free_pages:
             raise OutOfPages(f"{short} pages wanted, {pc.free_pages} free")
+        tokens = self._ids(tokens)
         for s, n in zip(seqs, need):
             pc.reserve(s, n)
         at = torch.tensor([[pc.lens[s] for s in seqs], list(seqs)])
         at = at.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else at
-        tokens = torch.as_tensor(tokens, dtype=torch.int64).to(dev)
         if self.graphs is None:
             logits = self._forward(tokens, at[0], pc.table[at[1]])
         else:

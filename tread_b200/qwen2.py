@@ -169,8 +169,8 @@ class Qwen2Rows:
 
     @torch.inference_mode()  # the words may have been made in it, and are then cleared in it only
     def check_errors(self):
-        """Raise if a kernel flagged an out-of-range row position: the row kernels' error word and
-        the selector's sticky flag, read with one device sync."""
+        """Raise if a kernel flagged an out-of-range row position (or a decode step a page or a token id): the row
+        kernels' error word and the selector's sticky flag, read with one device sync."""
         sel = kernels.selector_flags(self.device)
         e = int(torch.cat([self.err, sel]).max().item())
         if e:
@@ -178,5 +178,5 @@ class Qwen2Rows:
             sel.zero_()
             if e & 4:  # an attention kernel gave up on a wait: its split-tile counters may be stale
                 kernels.reset_attn_workspace(self.device)
-            raise RuntimeError(f"tread_b200 kernel reported an error (flags {e:#x}: 1, 2 out-of-range position, "
-                               f"4 wait timeout)")
+            raise RuntimeError(f"tread_b200 kernel reported an error (flags {e:#x}: 1, 2 out-of-range position, page "
+                               f"or token, 4 wait timeout)")
