@@ -21,6 +21,23 @@ def _bucket(n, T, n_min=64, n_step=256, t_step=1024):
     return nb, Tb
 
 
+def capture(body, device):
+    """(graph, body()'s result): `body` warmed up twice and captured, all on one stream of `device`, which need
+    not be the current device (torch.cuda.graph's own stream belongs to the device that was current when the
+    process captured first)."""
+    with torch.cuda.device(device):
+        s = torch.cuda.Stream(device=device)
+        s.wait_stream(torch.cuda.current_stream(device))
+        with torch.cuda.stream(s):
+            for _ in range(2):
+                body()
+        torch.cuda.current_stream(device).wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = body()
+    return graph, out
+
+
 class _Graph:
     def __init__(self, net, start, nb, Tb):
         L = net.L
@@ -35,15 +52,7 @@ class _Graph:
         def body():
             return net.run(self.h, self.pos, Ks, Vs, start)
 
-        s = torch.cuda.Stream(device=net.device)
-        s.wait_stream(torch.cuda.current_stream(net.device))
-        with torch.cuda.stream(s):
-            for _ in range(2):
-                body()
-        torch.cuda.current_stream(net.device).wait_stream(s)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.out = body()
+        self.graph, self.out = capture(body, net.device)
 
 
 class SubsetRunner:
@@ -137,13 +146,5 @@ class RequestGraph:
         def body():
             return compute(self.K, self.V, self.ctx, self.q, self.cands, T, nq, ratio, policy)
 
-        s = torch.cuda.Stream(device=net.device)
-        s.wait_stream(torch.cuda.current_stream(net.device))
-        with torch.cuda.stream(s):
-            for _ in range(2):
-                body()
-        torch.cuda.current_stream(net.device).wait_stream(s)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.logits, self.eff = body()
+        self.graph, (self.logits, self.eff) = capture(body, net.device)
         net.err.zero_()  # the warm-up ran on an all-zero cache

@@ -20,6 +20,7 @@ import torch
 
 from tread_b200 import kernels
 from tread_b200.blend import rows_of
+from tread_b200.graphs import capture
 
 
 class OutOfPages(RuntimeError):
@@ -263,12 +264,4 @@ class _StepGraph:
         self.tokens = torch.zeros(size, dtype=torch.int64, device=dev)
         self.pos = torch.full((size,), -1, dtype=torch.int64, device=dev)  # captured idle: nothing is appended
         self.table = torch.full((size, dec.cache.table.shape[1]), -1, dtype=torch.int32, device=dev)
-        s = torch.cuda.Stream(device=dev)
-        s.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(s):
-            for _ in range(2):
-                dec._forward(self.tokens, self.pos, self.table)
-        torch.cuda.current_stream(dev).wait_stream(s)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.logits = dec._forward(self.tokens, self.pos, self.table)
+        self.graph, self.logits = capture(lambda: dec._forward(self.tokens, self.pos, self.table), dev)
