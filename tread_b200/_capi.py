@@ -7,10 +7,10 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sysconfig
 
 import torch
 
-BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "tread_decode.so")
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libtread_b200.so")
 
 TREAD_F32, TREAD_F16, TREAD_BF16 = 0, 1, 2
@@ -103,6 +103,13 @@ def lib():
     return _lib
 
 
+def binding_path():
+    """The decode binding's file, named after what it is compiled against: PyTorch's and CPython's headers, whose
+    layouts change with their versions."""
+    tag = f"{sysconfig.get_config_var('SOABI')}-torch{torch.__version__}-abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    return os.path.join(os.path.dirname(LIB_PATH), f"tread_decode.{tag}.so")
+
+
 _binding = None
 
 
@@ -110,12 +117,13 @@ def binding():
     """The compiled binding of the decode-step operators (csrc/decode_binding.cpp), loaded once."""
     global _binding
     if _binding is None:
-        if not os.path.exists(BINDING_PATH):
-            raise RuntimeError(
-                f"tread_b200 decode binding not built ({BINDING_PATH} missing); run `python -m tread_b200.build`")
+        path = binding_path()
+        if not os.path.exists(path):
+            raise RuntimeError(f"tread_b200 decode binding not built for this Python and PyTorch ({path} missing); run "
+                               "`python -m tread_b200.build`")
         lib()
-        loader = importlib.machinery.ExtensionFileLoader("tread_decode", BINDING_PATH)
-        spec = importlib.util.spec_from_file_location("tread_decode", BINDING_PATH, loader=loader)
+        loader = importlib.machinery.ExtensionFileLoader("tread_decode", path)
+        spec = importlib.util.spec_from_file_location("tread_decode", path, loader=loader)
         _binding = importlib.util.module_from_spec(spec)
         loader.exec_module(_binding)
     return _binding

@@ -3,8 +3,9 @@
 Every `csrc/*.cu` is compiled with nvcc for `sm_100a` only and linked into one shared
 library with the CUDA runtime linked statically, so the `.so` has no dependency beyond the
 driver. `csrc/decode_binding.cpp`, the Python binding of the decode-step operators, is compiled with
-g++ against PyTorch's headers into `_lib/tread_decode.so` beside it. Both are built in-tree so that
-they travel with the source tree.
+g++ against PyTorch's headers into `_lib/tread_decode.<Python and PyTorch>.so` beside it; another
+version of either makes another file, and an old one is not loaded. Both are built in-tree so that they
+travel with the source tree.
 
     python -m tread_b200.build [-v] [--force]
 """
@@ -20,7 +21,6 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 LIB = os.path.join(OUT_DIR, "libtread_b200.so")
-BINDING = os.path.join(OUT_DIR, "tread_decode.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -69,13 +69,18 @@ def build(verbose=False, force=False, ptxas_verbose=False):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-    src = os.path.join(CSRC, "decode_binding.cpp")
-    if force or _stale(BINDING, [src, os.path.join(ROOT, "include", "tread_b200.h")]):
-        build_binding(src, verbose)
+    from tread_b200._capi import binding_path
+
+    src, binding = os.path.join(CSRC, "decode_binding.cpp"), binding_path()
+    for f in os.listdir(OUT_DIR):  # of another Python or PyTorch
+        if f.startswith("tread_decode.") and f != os.path.basename(binding):
+            os.remove(os.path.join(OUT_DIR, f))
+    if force or _stale(binding, [src, os.path.join(ROOT, "include", "tread_b200.h")]):
+        build_binding(src, binding, verbose)
     return LIB
 
 
-def build_binding(src, verbose=False):
+def build_binding(src, binding, verbose=False):
     import sysconfig
 
     import torch
@@ -87,7 +92,7 @@ def build_binding(src, verbose=False):
     lib = os.path.join(root, "lib")
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{d}" for d in include]
-    cmd += [src, "-o", BINDING, f"-L{OUT_DIR}", f"-L{lib}", "-ltread_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+    cmd += [src, "-o", binding, f"-L{OUT_DIR}", f"-L{lib}", "-ltread_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu",
             "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
