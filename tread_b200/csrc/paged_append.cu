@@ -149,15 +149,18 @@ template <typename T>
 int launch(const AppendArgs& a, bool vec, cudaStream_t st) {
   constexpr int VEC = 16 / sizeof(T);
   const int hv = (a.D / 2) / (vec ? VEC : 1), places = kThreads / hv;
+  int device = 0, sms = 0;
+  TREAD_CHECK_CUDA(cudaGetDevice(&device));
+  TREAD_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
   // a CTA's places are rows first (each row's cosines are then found once), as far as there are rows for eight
   // CTAs an SM, then heads. Rows for two an SM take 81 us instead of 79 at 16640 rows of 56 heads of 128, and
   // heads split until an SM has eight CTAs instead of four, 86.
   int tile_log2 = 0;
-  while ((2 << tile_log2) <= places && (2 << tile_log2) <= kMaxTile && (a.R >> (tile_log2 + 1)) >= 1184) ++tile_log2;
+  while ((2 << tile_log2) <= places && (2 << tile_log2) <= kMaxTile && (a.R >> (tile_log2 + 1)) >= 8 * sms) ++tile_log2;
   const long long tiles = ((long long)a.R + (1 << tile_log2) - 1) >> tile_log2;
   const int lanes = places >> tile_log2;
   const long long passes = (a.Hq + 2LL * a.Hkv + lanes * kUnroll - 1) / (lanes * kUnroll);
-  long long split = (592 + tiles - 1) / tiles;
+  long long split = (4 * sms + tiles - 1) / tiles;
   if (split > passes) split = passes;
   dim3 grid((unsigned)tiles, (unsigned)split);
   if (vec)
