@@ -300,7 +300,8 @@ int tread_paged_append(const tread_paged_append_args* args, tread_stream_t strea
  *           a score above -inf, or there is none, the output is zero
  * A length below 0 or above max_pages * page_size gives a row of zeros; keys in a page whose id is
  * outside the pool count as masked. Both set bit 1 of *err_flag (may be NULL). What slots behind a
- * sequence's length hold does not matter. D in {64, 128, 256}, Hq / Hkv at most 16; q, out, the pools,
+ * sequence's length hold does not matter. An infinite value of a key that counts gives an output that is not
+ * finite (in 16-bit types, whose weights come in two parts, possibly NaN). D in {64, 128, 256}, Hq / Hkv at most 16; q, out, the pools,
  * and rows, heads and pages of them on 16-byte boundaries; max_pages * page_size below 2^31 - 16, and
  * Hkv * B * max_pages * page_size below about 2^34.
  * workspace: tread_paged_attn_workspace_bytes() of device memory, 256-byte aligned, contents

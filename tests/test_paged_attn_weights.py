@@ -183,3 +183,25 @@ def test_fp16_scores_whose_steps_are_wide():
     vp = torch.randn(pool, 1, page, D, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).to(HF)
     got = kernels.paged_attn(q, kp, vp, table.expand(B, -1), torch.full((B,), n, device="cuda"), sm_scale=2.0 ** 13)
     assert bool(got.isfinite().all()) and float(got.abs().max()) <= float(vp.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_infinite_values_stay_in_their_element(dtype):
+    """Not finite in the element and the heads that read it, whatever the weight's two parts are; the others as
+    without it."""
+    g = torch.Generator("cuda").manual_seed(3)
+    table, pool = make_table([100], 16, g)
+    q = torch.randn(1, 8, 64, device="cuda", generator=g).to(dtype)
+    kp, vp = (torch.randn(pool, 2, 16, 64, device="cuda", generator=g).to(dtype) for _ in range(2))
+    lens = torch.tensor([100], device="cuda")
+    want = kernels.paged_attn(q, kp, vp, table, lens)
+    for sign in (1, -1):
+        v2 = vp.clone()
+        v2[table[0, 3].long(), 1, 5, 9] = sign * torch.inf
+        got = kernels.paged_attn(q, kp, v2, table, lens)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[0, 4:, 9] = True
+        assert torch.equal(got.isfinite(), ~hit) and torch.equal(got[~hit], want[~hit])
+        if dtype == FP:
+            assert bool((got[hit] == sign * torch.inf).all())

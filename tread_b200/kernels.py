@@ -516,8 +516,10 @@ def paged_attn(q, k_pages, v_pages, table, lens, out=None, sm_scale=None, err=No
     has a score above -inf, or there is none (length 0), the output is zero.
     D in {64, 128, 256}, Hq / Hkv at most 16; q's rows, heads and pages on 16-byte boundaries; any page
     size (multiples of 16 are read without a lookup per key). What slots behind a length hold does not
-    matter. err: device error word; a length that the table has no pages for gives a row of zeros and
-    sets bit 1; a page id outside the pool sets it too, and its keys count as masked.
+    matter. An infinite value of a key that counts gives an output that is not finite (in 16-bit types,
+    which take a weight in two parts, possibly NaN). err: device error word; a length that the table has no
+    pages for gives a row of zeros and sets bit 1; a page id outside the pool sets it too, and its keys
+    count as masked.
     Returns out [B, Hq, D] (out may be q itself, and else does not overlap it)."""
     if stream is not None:
         with _on_stream(stream, k_pages):

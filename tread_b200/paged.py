@@ -119,7 +119,10 @@ class PagedDecoder:
     """Decode steps of a model (or its rows: Qwen2Rows, TPQwen2Rows) over a PagedCache.
 
     graphs=True captures one CUDA graph per batch size (powers of two up to `max_seqs`); a step of fewer
-    sequences pads the batch with rows of position -1, which append nothing and attend to nothing."""
+    sequences pads the batch with rows of position -1, which append nothing and attend to nothing.
+
+    Used from one stream at a time, as the engine is: the rows' projections share a workspace (eager steps,
+    captured ones and other decoders of the same device alike)."""
 
     def __init__(self, model, num_pages, page_size=64, max_seqs=64, max_len=32768, graphs=False):
         net = self.net = rows_of(model)
